@@ -38,6 +38,10 @@ THREAD_HEADERS = THREAD_HEADERS + [os.path.join(PKG, "scenes", "b3_test_forces.h
 THREAD_DEPS = THREAD_HEADERS + [os.path.join(ROOT, "include", "puffysics_b200.h"),
                                 os.path.join(PKG, "csrc", "b3x_math.cuh"), os.path.join(PKG, "csrc", "b3x_narrow.cuh"),
                                 os.path.join(PKG, "scenes", "b3_scenes.h")]
+# the training operators (libb3train.so)
+TRAIN_SRC = [os.path.join(PKG, "csrc", "b3x_train_%s.cu" % n) for n in ("logprob", "advantage", "adamw")]
+TRAIN_LIB = os.path.join(LIB_DIR, "libb3train.so")
+TRAIN_HEADERS = [os.path.join(ROOT, "include", "b3x_train.h"), os.path.join(PKG, "csrc", "b3x_train_common.cuh")]
 # capacity configurations the host scene builders are compiled for:
 # name -> (bodies, shapes, contacts, joints)
 SCENE_CONFIGS = {"hover": (2, 2, 4, 1), "stack": (9, 9, 32, 1), "chain": (12, 12, 32, 10),
@@ -105,14 +109,24 @@ def hover_cmd():
                "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(PKG, "csrc"), HOVER_SRC, "-o", HOVER_LIB])
 
 
+def train_cmd(extra=()):
+    return ([NVCC] + ARCH + ["-lineinfo", "-O3", "-std=c++17"] + PARITY
+            + ["-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-cudart", "static", "--threads", "0",
+               "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(PKG, "csrc")]
+            + list(extra) + TRAIN_SRC + ["-o", TRAIN_LIB])
+
+
 def build_thread_libs(force=False):
-    """The per-thread step launchers, one per capacity configuration, and the
-    hover environment library, compiled concurrently."""
+    """The per-thread step launchers, one per capacity configuration, the
+    hover environment library and the training operators, compiled
+    concurrently."""
     deps = [THREAD_SRC, __file__] + THREAD_DEPS
     todo = [n for n in thread_lib_names() if force or _newer(thread_lib(n), deps)]
     cmds = {n: thread_cmd(n) for n in todo}
     if force or _newer(HOVER_LIB, [HOVER_SRC, __file__] + THREAD_DEPS + HOVER_HEADERS):
         cmds["hover environment"] = hover_cmd()
+    if force or _newer(TRAIN_LIB, TRAIN_SRC + TRAIN_HEADERS + [__file__]):
+        cmds["training operators"] = train_cmd()
     procs = [(n, subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
              for n, c in cmds.items()]
     errors = []
@@ -140,7 +154,8 @@ def up_to_date():
     thread_deps = [THREAD_SRC, __file__] + THREAD_DEPS
     return (not _newer(LIB, deps) and not any(_newer(scenes_lib(n), [SCENES_SRC] + HEADERS) for n in SCENE_CONFIGS)
             and not any(_newer(thread_lib(n), thread_deps) for n in thread_lib_names())
-            and not _newer(HOVER_LIB, [HOVER_SRC, __file__] + THREAD_DEPS + HOVER_HEADERS))
+            and not _newer(HOVER_LIB, [HOVER_SRC, __file__] + THREAD_DEPS + HOVER_HEADERS)
+            and not _newer(TRAIN_LIB, TRAIN_SRC + TRAIN_HEADERS + [__file__]))
 
 
 def build_scenes(force=False):

@@ -1,0 +1,47 @@
+// b3x_train_common.cuh -- element types and arithmetic shared by the training
+// operators (include/b3x_train.h).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "b3x_train.h"
+
+namespace b3t {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInf = __builtin_huge_valf();
+
+template <class T> __device__ __forceinline__ float to_float(T x) { return (float)x; }
+template <> __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+template <class T> __device__ __forceinline__ T from_float(float x) { return (T)x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float(float x) { return __float2half_rn(x); }
+
+// 2^x; about 2 ulp, results under the normal range are 0.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+
+// Whether (rows, cols) elements at these strides are apart from one another.
+inline bool apart(long long rows, long long cols, long long rs, long long cs) {
+    if (rows < 2 && cols < 2) return true;
+    if (rows < 2) return cs > 0;
+    if (cols < 2) return rs > 0;
+    if (rs <= 0 || cs <= 0) return false;
+    return rs >= cs ? (rs - 1) / cs >= cols - 1 : (cs - 1) / rs >= rows - 1;
+}
+
+}  // namespace b3t
