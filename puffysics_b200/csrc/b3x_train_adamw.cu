@@ -57,11 +57,6 @@ __host__ __device__ __forceinline__ unsigned mix(unsigned x) {
     return x ^ (x >> 16);
 }
 
-template <class T> struct TypeId;
-template <> struct TypeId<float> { static constexpr int value = B3X_F32; };
-template <> struct TypeId<__nv_bfloat16> { static constexpr int value = B3X_BF16; };
-template <> struct TypeId<__half> { static constexpr int value = B3X_F16; };
-
 // e4m3 codes of x / scale.  Scaled by 2^-120 the format's exponents are
 // float's, subnormals included, so the code is the upper bits of the word; what
 // is added to the 20 bits below it rounds.
@@ -118,7 +113,7 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         if (!kF8) ((float*)t.m)[i] = m[k], ((float*)t.v)[i] = v;
         float p = to_float(((P*)t.p)[i]) * t.keep - (m[k] / (r[k] * h.root + h.eps)) * h.rate;
         if (t.copy) t.copy[i] = __float2bfloat16_rn(p);
-        if (TypeId<P>::value == B3X_BF16 && stochastic && fabsf(p) < kInf) {
+        if (sizeof(P) == 2 && stochastic && fabsf(p) < kInf) {
             const unsigned low = mix(mix((unsigned)i * 0x9E3779B1u + (unsigned)(i >> 32) * 0x6A09E667u + t.key) + 0x9E3779B1u);
             p = __uint_as_float((__float_as_uint(p) + (low & 0xFFFFu)) & 0xFFFF0000u);
         }
