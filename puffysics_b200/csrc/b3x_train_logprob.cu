@@ -55,37 +55,65 @@ __device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t index) {
 __device__ __forceinline__ int index_of(uint64_t e) { return (int)(0xFFFFFFFFu - (uint32_t)e); }
 
 // ---- running sums -----------------------------------------------------------------------
-// What a part of a row comes to: its maximum m, s = sum 2^x and t = sum x 2^x with
-// x = c (z - m), c = scale log2 e.  Joined parts move to the larger maximum:
-// 2^(x + d) (x + d) = 2^d (2^x x + d 2^x).  Exponents stop at -1e4, where 2^x is 0
-// already, so that -infinity (d of an empty part, x of a masked logit) never
-// meets a zero factor.  A NaN maximum stays; sums beside it mean nothing.
+// What a part of a row comes to: its maximum m, a whole number r near c m
+// (c = scale log2 e), s = sum 2^x and t = sum x 2^x with x = c z - r.  r is
+// exact, so one fused operation gives x with a rounding of its own size only,
+// and what c's rounding does to c z it does to c m as well:
+//   L = ln s - ln 2 (c m - r),  H = ln s - ln 2 t / s.
+// Joined parts move to the larger r: 2^(x + d) (x + d) = 2^d (2^x x + d 2^x).
+// Shifts and exponents stop at -1e4, where 2^x is 0 already, so that -infinity
+// never meets a zero factor.  A NaN maximum stays; sums beside it mean nothing.
 struct Part {
-    float m, s, t;
+    float m, r, s, t;
 };
+__device__ __forceinline__ Part empty_part() { return Part{-kInf, -3.0e38f, 0.0f, 0.0f}; }
 
-__device__ __forceinline__ Part join(Part a, Part b, float c) {
-    const float m = max_nan(a.m, b.m);
-    const float da = fmaxf((a.m - m) * c, -1e4f), db = fmaxf((b.m - m) * c, -1e4f);
-    const float fa = exp2_fast(da), fb = exp2_fast(db);
-    return Part{m, a.s * fa + b.s * fb, __fmaf_rn(fa, __fmaf_rn(da, a.s, a.t), fb * __fmaf_rn(db, b.s, b.t))};
+__device__ __forceinline__ float reference(float m, float c) { return fminf(fmaxf(rintf(m * c), -3.0e38f), 3.0e38f); }
+
+__device__ __forceinline__ Part moved(Part a, float m, float r) {
+    const float d = fmaxf(a.r - r, -1e4f), f = exp2_fast(d);
+    return Part{m, r, a.s * f, f * __fmaf_rn(d, a.s, a.t)};
 }
 
-__device__ __forceinline__ Part join_lanes(Part a, float c, int lanes) {
-    for (int o = lanes / 2; o; o >>= 1)
-        a = join(a, Part{__shfl_xor_sync(~0u, a.m, o), __shfl_xor_sync(~0u, a.s, o), __shfl_xor_sync(~0u, a.t, o)}, c);
+// A warp's maximum, keeping a NaN.
+__device__ __forceinline__ float warp_max(float x) {
+    float y;
+    asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ Part join_lanes(Part a) {
+    a = moved(a, warp_max(a.m), warp_max(a.r));
+    for (int o = 16; o; o >>= 1) a.s += __shfl_xor_sync(~0u, a.s, o), a.t += __shfl_xor_sync(~0u, a.t, o);
     return a;
 }
+
+// Whether c m went beyond the floats (logits of 1e38): the row needs sums of (z - m) instead.
+__device__ __forceinline__ bool out_of_range(const Part& a) {
+    return fabsf(a.m) < kInf && !(a.s >= 0.5f && a.s < 1e30f);
+}
+
+constexpr float kLn2 = 0.6931471805599453f;
 
 // A row's results from its sums.
 struct Row {
     float m, logsum, entropy;
-    __device__ __forceinline__ explicit Row(Part a) {
+    __device__ __forceinline__ Row(Part a, float c) {
         const bool empty = a.m == -kInf;
         const float bad = empty ? 0.0f : a.m - a.m;   // NaN where the maximum is no number
         m = a.m;
-        logsum = empty ? 0.0f : logf(a.s) + bad;
-        entropy = empty ? 0.0f : logsum - 0.6931471805599453f * (a.t / a.s);
+        const float log_s = logf(a.s);
+        logsum = empty ? 0.0f : __fmaf_rn(-kLn2, __fmaf_rn(a.m, c, -a.r), log_s) + bad;
+        entropy = empty ? 0.0f : __fmaf_rn(-kLn2, a.t / a.s, log_s) + bad;
+    }
+    // The same where x was c (z - m): r is c m itself.
+    static __device__ __forceinline__ Row about_maximum(Part a) {
+        a.r = 0.0f;
+        const float m = a.m;
+        a.m = m == -kInf || m - m != 0.0f ? m : 0.0f;
+        Row row(a, 0.0f);
+        row.m = m;
+        return row;
     }
     __device__ __forceinline__ float logp(float z, float scale) const {
         return z == -kInf && m == -kInf ? -kInf : (z - m) * scale - logsum;
@@ -123,7 +151,7 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(Rows a, Out o) {
     }
     for (int k = L / 2; k; k >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, k));
     const float c = a.scale * kLog2e;
-    Part p{m, 0.0f, 0.0f};
+    Part p{m, 0.0f, 0.0f, 0.0f};   // the maximum is known before the sums: x = c (z - m)
 #pragma unroll
     for (int i = 0; i < kShort; i++) {
         const float x = fmaxf((z[i] - m) * c, -1e4f), e = exp2_fast(x);
@@ -131,7 +159,7 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(Rows a, Out o) {
         p.t = __fmaf_rn(e, x, p.t);
     }
     for (int k = L / 2; k; k >>= 1) p.s += __shfl_xor_sync(~0u, p.s, k), p.t += __shfl_xor_sync(~0u, p.t, k);
-    const Row r(p);
+    const Row r = Row::about_maximum(p);
     if (on && lane == 0) write_row<T>(a, o, row, r);
     uint64_t last = ~0ull;
     for (int k = 0; k < o.top; k++) {
@@ -189,6 +217,16 @@ struct Source {
     }
     __device__ __forceinline__ int vectors() const { return (head + width + Vec<T>::n - 1) / Vec<T>::n; }
 
+    // Vectors [2, last) and two words beside them are inside the row.
+    __device__ __forceinline__ int last() const { return (head + width) / Vec<T>::n - 1; }
+    // A vector among those.
+    __device__ __forceinline__ uint4 inner(int v) const {
+        const int j = v * Vec<T>::n - head;
+        uint4 q = load16(row + j);
+        if (kMask) keep(q, mask + j);
+        return q;
+    }
+
     // Vector v, -infinity where it is outside the row or masked.
     __device__ __forceinline__ uint4 load(int v) const {
         constexpr int N = Vec<T>::n;
@@ -211,34 +249,40 @@ struct Source {
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
 
+    // Mask bytes j on, where the words around them may lie outside the row's own.
     __device__ __forceinline__ void apply(uint4& q, int j) const {
         constexpr int N = Vec<T>::n;
-        const unsigned char* p = mask + j;
-        const int off = (int)((uintptr_t)p & 3);
-        uint32_t b[2];
-        // whole words around the N bytes, where they stay inside the row's own
-        if (j >= off && j - off + N + 4 <= width) {
-            const uint32_t* w = reinterpret_cast<const uint32_t*>(p - off);
-            const uint32_t w0 = __ldg(w), w1 = N == 8 || off ? __ldg(w + 1) : 0u, w2 = N == 8 && off ? __ldg(w + 2) : 0u;
-            b[0] = __funnelshift_r(w0, w1, off * 8);
-            b[1] = __funnelshift_r(w1, w2, off * 8);
-        } else {
-            b[0] = b[1] = 0;
+        const int off = (int)((uintptr_t)(mask + j) & 3);
+        if (j >= off && j - off + N + 4 <= width) return keep(q, mask + j);
+        uint32_t b[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < N; i++) b[i / 4] |= (uint32_t)p[i] << i % 4 * 8;
-        }
+        for (int i = 0; i < N; i++) b[i / 4] |= (uint32_t)mask[j + i] << i % 4 * 8;
+        keep(q, b);
+    }
+
+    // The N mask bytes at p, from the whole words around them.
+    static __device__ __forceinline__ void keep(uint4& q, const unsigned char* p) {
+        constexpr int N = Vec<T>::n;
+        const int off = (int)((uintptr_t)p & 3);
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(p - off);
+        const uint32_t w0 = __ldg(w), w1 = N == 8 || off ? __ldg(w + 1) : 0u, w2 = N == 8 && off ? __ldg(w + 2) : 0u;
+        uint32_t b[2] = {__funnelshift_r(w0, w1, off * 8), __funnelshift_r(w1, w2, off * 8)};
+        keep(q, b);
+    }
+
+    static __device__ __forceinline__ void keep(uint4& q, uint32_t (&b)[2]) {
         uint32_t* w = &q.x;
         b[0] = nonzero_bytes(b[0]);
-        if (N == 4) {
+        if (Vec<T>::n == 4) {
 #pragma unroll
             for (int i = 0; i < 4; i++) w[i] = b[0] >> i * 8 & 0x80u ? w[i] : minus_infinity<T>();
         } else {
             b[1] = nonzero_bytes(b[1]);
 #pragma unroll
             for (int i = 0; i < 4; i++) {   // a byte's sign bit becomes 16 bits of ones
-                uint32_t keep;
-                asm("prmt.b32 %0, %1, 0, %2;" : "=r"(keep) : "r"(b[i / 2]), "r"(i % 2 ? 0xBBAA : 0x9988));
-                w[i] = (w[i] & keep) | (minus_infinity<T>() & ~keep);
+                uint32_t ones;
+                asm("prmt.b32 %0, %1, 0, %2;" : "=r"(ones) : "r"(b[i / 2]), "r"(i % 2 ? 0xBBAA : 0x9988));
+                w[i] = (w[i] & ones) | (minus_infinity<T>() & ~ones);
             }
         }
     }
@@ -294,34 +338,194 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     uint64_t r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
 
+// U vectors' part of s and t.  What is -infinity is known only by the NaN it
+// leaves in t (0 times -infinity): then, and always with a mask, once more with
+// the exponents stopped, which costs an instruction a logit.
+template <class T, int U, bool kMask>
+__device__ __forceinline__ void add_vectors(const uint4 (&q)[U], float c, Part& p) {
+    constexpr int N = Vec<T>::n;
+    const uint64_t by = pack2(c, c), minus = pack2(-p.r, -p.r);
+    uint64_t s2, t2;
+    auto go = [&](bool stop) {
+        s2 = t2 = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int i = 0; i < N / 2; i++) {
+                float2 x = unpack2(fma2(pack2(element<T>(q[u], 2 * i), element<T>(q[u], 2 * i + 1)), by, minus));
+                if (stop) x.x = fmaxf(x.x, -1e4f), x.y = fmaxf(x.y, -1e4f);
+                const uint64_t e = pack2(exp2_fast(x.x), exp2_fast(x.y));
+                s2 = add2(s2, e);
+                t2 = fma2(e, pack2(x.x, x.y), t2);
+            }
+        }
+    };
+    go(kMask);
+    float2 t = unpack2(t2);
+    if (!kMask && t.x + t.y != t.x + t.y) {
+        go(true);
+        t = unpack2(t2);
+    }
+    const float2 s = unpack2(s2);
+    p.s += s.x + s.y;
+    p.t += t.x + t.y;
+}
+
+template <class T, int U>
+__device__ __forceinline__ float most_of(const uint4 (&q)[U]) {
+    float m = most<T>(q[0]);
+#pragma unroll
+    for (int u = 1; u < U; u++) m = max_nan(m, most<T>(q[u]));
+    return m;
+}
+
+template <class T> __device__ __forceinline__ uint4 no_vector() {
+    return make_uint4(minus_infinity<T>(), minus_infinity<T>(), minus_infinity<T>(), minus_infinity<T>());
+}
+
+// The lanes' keys from the largest down.
+__device__ __forceinline__ uint32_t sort_lanes(uint32_t key) {
+    const int lane = threadIdx.x % 32;
+#pragma unroll
+    for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+        for (int j = k / 2; j; j /= 2) {
+            const uint32_t other = __shfl_xor_sync(~0u, key, j);
+            const bool larger = ((lane & j) == 0) == ((lane & k) == 0);
+            key = larger ? max(key, other) : min(key, other);
+        }
+    return key;
+}
+
+__device__ __forceinline__ void write_top(const Out& o, long long row, int k, uint64_t e, const Row& r, float scale) {
+    o.top_ids[row * o.top + k] = e ? index_of(e) : -1;
+    o.top_logp[row * o.top + k] = e ? r.logp(of_key((uint32_t)(e >> 32)), scale) : -kInf;
+}
+
+// The sums of a row of logits of 1e38, whose products with c are beyond the
+// floats: x = c (z - m).  `by`: threads that share the row.
+template <class T, bool kMask>
+__device__ __noinline__ float2 far_sums(const Source<T, kMask>& src, float m, float c, int first, int by) {
+    float s = 0.0f, t = 0.0f;
+    for (int v = first; v < src.vectors(); v += by) {
+        const uint4 q = src.load(v);
+        for (int n = 0; n < Vec<T>::n; n++) {
+            const float x = fmaxf((element<T>(q, n) - m) * c, -1e4f), e = exp2_fast(x);
+            s += e;
+            t = __fmaf_rn(e, x, t);
+        }
+    }
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o), t += __shfl_xor_sync(~0u, t, o);
+    return make_float2(s, t);
+}
+
+// ---- rows of a warp -----------------------------------------------------------------------
+// Rows of up to 32 U vectors, one a warp, kept in registers.  The K-th largest of
+// the lanes' maxima is at most the K-th largest logit: what reaches it is ranked.
+constexpr int kRowWarps = 8;
+constexpr int kRowFound = 160;
+
+template <class T, bool kMask, bool kTop, int U>
+__global__ void __launch_bounds__(kRowWarps * 32) row_kernel(Rows a, Out o) {
+    constexpr int N = Vec<T>::n;
+    __shared__ uint64_t entries[kTop ? kRowWarps : 1][kTop ? kRowFound : 1];
+    __shared__ int found[kRowWarps];
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const long long row = (long long)blockIdx.x * kRowWarps + warp;
+    if (row >= a.rows) return;
+    const Source<T, kMask> src(a, row);
+    const int nv = src.vectors();
+    const float c = a.scale * kLog2e;
+    uint4 q[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) q[u] = u * 32 + lane < nv ? src.load(u * 32 + lane) : no_vector<T>();
+    const float mine = most_of<T, U>(q);
+    Part p = empty_part();
+    p.m = warp_max(mine);
+    p.r = reference(p.m, c);
+    add_vectors<T, U, kMask>(q, c, p);
+    for (int k = 16; k; k >>= 1) p.s += __shfl_xor_sync(~0u, p.s, k), p.t += __shfl_xor_sync(~0u, p.t, k);
+    const bool far = out_of_range(p);
+    if (far) {
+        const float2 st = far_sums(src, p.m, c, lane, 32);
+        p.s = st.x, p.t = st.y;
+    }
+    const Row r = far ? Row::about_maximum(p) : Row(p, c);
+    if (lane == 0) write_row<T>(a, o, row, r);
+    if (!kTop) return;
+    const uint32_t sorted = sort_lanes(key_of(mine));
+    const uint32_t threshold = max(__shfl_sync(~0u, sorted, o.top - 1), kNothing + 1);
+    if (lane == 0) found[warp] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        if (key_of(most<T>(q[u])) < threshold) continue;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const uint32_t key = key_of(element<T>(q[u], n));
+            if (key < threshold) continue;
+            const int at = atomicAdd(&found[warp], 1);
+            if (at < kRowFound) entries[warp][at] = entry_of(key, (u * 32 + lane) * N - src.head + n);
+        }
+    }
+    __syncwarp();
+    const int n = found[warp];
+    if (n <= kRowFound && p.m == p.m) {
+        for (int i = lane; i < n; i += 32) {
+            const uint64_t e = entries[warp][i];
+            int rank = 0;
+            for (int j = 0; j < n; j++) rank += entries[warp][j] > e;
+            if (rank < o.top) write_top(o, row, rank, e, r, a.scale);
+        }
+        if (lane >= n && lane < o.top) write_top(o, row, lane, 0, r, a.scale);
+        return;
+    }
+    // many equal logits, or NaN: each time the best one after the last
+    uint64_t last = ~0ull;
+    for (int k = 0; k < o.top; k++) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            for (int i = 0; i < N; i++) {
+                const uint32_t key = key_of(element<T>(q[u], i));
+                const uint64_t e = entry_of(key, (u * 32 + lane) * N - src.head + i);
+                if (key > kNothing && key <= kMost && e < last && e > best) best = e;
+            }
+        for (int d = 16; d; d >>= 1) {
+            const uint64_t other = __shfl_xor_sync(~0u, best, d);
+            best = other > best ? other : best;
+        }
+        last = best;
+        if (lane == 0) write_top(o, row, k, best, r, a.scale);
+    }
+}
+
+// ---- rows of a block or a cluster ------------------------------------------------------------
 constexpr int kUnroll = 4;           // vectors a thread has in flight
+constexpr int kTile = 32 * kUnroll;  // vectors a warp takes at a time
 constexpr int kGroups = 256;         // groups of consecutive vectors whose maxima are kept
 constexpr int kFound = 512;          // logits at or above the threshold that are ranked at once
 constexpr int kMaxWarps = 16;
 constexpr int kMaxCluster = 8;
 
 struct Shared {
-    float m[kMaxWarps], s[kMaxWarps], t[kMaxWarps];
-    Part part;                        // this block's
-    Part joined;
+    Part part[kMaxWarps];
+    Part all;                         // this block's
     uint32_t group[kGroups];
     int order[B3X_TRAIN_MAX_TOP];
     uint32_t threshold;
+    uint32_t largest[kMaxWarps], share[kMaxWarps];
     int found;
     uint64_t list[B3X_TRAIN_MAX_TOP]; // this block's alternatives
     uint64_t entries[kFound];
     uint64_t warp_best[kMaxWarps];
+    float2 far[kMaxWarps];
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -339,12 +543,13 @@ __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
     asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
     return w;
 }
+__device__ __forceinline__ float remote_float(const void* p, uint32_t rank) { return __uint_as_float(remote(p, rank)); }
 
 // The K largest entries among the vectors of some groups (or all): each time
 // the best one after the last.  Only for rows with many equal logits or NaN.
 template <class T, bool kMask>
-__device__ void search(const Source<T, kMask>& src, Shared& sh, int v0, int v1, int shift, const int* order, int groups,
-                       int top) {
+__device__ __noinline__ void search(const Source<T, kMask>& src, Shared& sh, int v0, int v1, int shift, const int* order,
+                                    int groups, int top) {
     const int warps = blockDim.x / 32;
     uint64_t last = ~0ull;
     for (int k = 0; k < top; k++) {
@@ -383,16 +588,31 @@ __device__ __forceinline__ void rank_entries(const uint64_t* entries, int n, int
     for (int i = n + threadIdx.x; i < top; i += blockDim.x) list[i] = 0;
 }
 
-// One block, or one cluster of blocks, a row.  Each warp takes kUnroll vectors a
-// lane at a time and keeps the maximum, sum and weighted sum of each lane
-// running; so a row is read once.  For the alternatives the maxima of groups of
-// 2^shift consecutive vectors are kept beside.  The K groups with the largest
-// maxima (the first among equal ones) hold the K largest logits, and the K-th of
-// those maxima is at most the K-th largest logit: those groups are read again,
-// from L2, and what reaches the threshold is ranked.
-template <class T, bool kMask, bool kTop, int kThreads>
-__global__ void __launch_bounds__(kThreads) long_kernel(Rows a, Out o, int cluster, int shift) {
-    constexpr int N = Vec<T>::n;
+// Adds a vector's logits that reach the threshold to the entries.
+template <class T, bool kMask>
+__device__ __forceinline__ void gather(const Source<T, kMask>& src, Shared& sh, const uint4& q, int v, uint32_t threshold) {
+    if (key_of(most<T>(q)) < threshold) return;
+#pragma unroll
+    for (int n = 0; n < Vec<T>::n; n++) {
+        const uint32_t key = key_of(element<T>(q, n));
+        if (key < threshold) continue;
+        const int at = atomicAdd(&sh.found, 1);
+        if (at < kFound) sh.entries[at] = entry_of(key, v * Vec<T>::n - src.head + n);
+    }
+}
+
+// One block, or one cluster of blocks, a row; the row is read once.  kOnce: each
+// warp has one tile, which stays in its registers.  Otherwise the warps walk
+// over the row with their sums running.
+//
+// Alternatives.  kOnce: a threshold that K logits reach, from the lanes' sorted
+// maxima: the K-th of any warp's, or the least of every warp's (K / warps)-th.
+// Otherwise the maxima of groups of 2^shift consecutive vectors are kept.  The K
+// groups with the largest maxima (the first among equal ones) hold the K largest
+// logits, and the K-th of those maxima is at most the K-th largest logit: those
+// groups are read again, from L2.  What reaches the threshold is ranked.
+template <class T, bool kMask, bool kTop, bool kOnce>
+__global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, int cluster, int shift) {
     __shared__ Shared sh;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const int rank = cluster > 1 ? (int)cluster_rank() : 0;
@@ -403,93 +623,105 @@ __global__ void __launch_bounds__(kThreads) long_kernel(Rows a, Out o, int clust
     const int v0 = min(nv, each * rank), v1 = min(nv, v0 + each);
     const float c = a.scale * kLog2e;
     if (kTop) {
-        for (int i = threadIdx.x; i < kGroups; i += blockDim.x) sh.group[i] = 0;
+        if (!kOnce)
+            for (int i = threadIdx.x; i < kGroups; i += blockDim.x) sh.group[i] = 0;
         if (threadIdx.x == 0) sh.found = 0;
         __syncthreads();
     }
 
-    Part p{-kInf, 0.0f, 0.0f};
-    for (int base = v0 + warp * 32 * kUnroll; base < v1; base += warps * 32 * kUnroll) {
-        uint4 q[kUnroll];
+    uint4 q[kUnroll];
+    Part p = empty_part();
+    for (int base = v0 + warp * kTile; base < v1 || kOnce; base += warps * kTile) {
+        if (base >= 2 && base + kTile <= min(v1, src.last())) {
 #pragma unroll
-        for (int u = 0; u < kUnroll; u++) {
-            const int v = base + u * 32 + lane;
-            q[u] = make_uint4(minus_infinity<T>(), minus_infinity<T>(), minus_infinity<T>(), minus_infinity<T>());
-            if (v < v1) q[u] = src.load(v);
+            for (int u = 0; u < kUnroll; u++) q[u] = src.inner(base + u * 32 + lane);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kUnroll; u++) {
+                const int v = base + u * 32 + lane;
+                q[u] = v < v1 ? src.load(v) : no_vector<T>();
+            }
         }
         float top[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; u++) top[u] = most<T>(q[u]);
         const float here = max_nan(max_nan(top[0], top[1]), max_nan(top[2], top[3]));
-        if (kTop) {
+        if (kTop && !kOnce) {
             if (shift >= 7) {
                 const uint32_t key = __reduce_max_sync(~0u, key_of(here));
                 if (lane == 0) atomicMax(&sh.group[(base - v0) >> shift], key);
-            } else {
+            } else {   // 5: a group is a warp's vectors of one u
 #pragma unroll
                 for (int u = 0; u < kUnroll; u++) {
-                    uint32_t key = key_of(top[u]);
-                    for (int k = 0; k < shift; k++) key = max(key, __shfl_xor_sync(~0u, key, 1 << k));
-                    const int v = base - v0 + u * 32 + lane;
-                    if ((lane & ((1 << shift) - 1)) == 0 && v < v1 - v0) sh.group[v >> shift] = key;
+                    const uint32_t key = __reduce_max_sync(~0u, key_of(top[u]));
+                    if (lane == 0 && base + u * 32 < v1) sh.group[(base - v0) / 32 + u] = key;
                 }
             }
         }
         const float m = max_nan(p.m, here);
-        const float d = fmaxf((p.m - m) * c, -1e4f), f = exp2_fast(d);
-        p = Part{m, p.s * f, f * __fmaf_rn(d, p.s, p.t)};
-        const uint64_t minus = pack2(-m, -m), by = pack2(c, c);
-        uint64_t s2 = 0, t2 = 0;
-#pragma unroll
-        for (int u = 0; u < kUnroll; u++) {
-#pragma unroll
-            for (int i = 0; i < N / 2; i++) {
-                const float2 z = make_float2(element<T>(q[u], 2 * i), element<T>(q[u], 2 * i + 1));
-                float2 x = unpack2(mul2(add2(pack2(z.x, z.y), minus), by));
-                x.x = fmaxf(x.x, -1e4f), x.y = fmaxf(x.y, -1e4f);
-                const uint64_t e = pack2(exp2_fast(x.x), exp2_fast(x.y));
-                s2 = add2(s2, e);
-                t2 = fma2(e, pack2(x.x, x.y), t2);
-            }
-        }
-        const float2 s = unpack2(s2), t = unpack2(t2);
-        p.s += s.x + s.y;
-        p.t += t.x + t.y;
+        p = moved(p, m, reference(m, c));
+        add_vectors<T, kUnroll, kMask>(q, c, p);
+        if (kOnce) break;
     }
-    p = join_lanes(p, c, 32);
-    if (lane == 0) sh.m[warp] = p.m, sh.s[warp] = p.s, sh.t[warp] = p.t;
+    const float mine = p.m;
+    p = join_lanes(p);
+    if (lane == 0) sh.part[warp] = p;
+    if (kTop && kOnce) {
+        const uint32_t sorted = sort_lanes(key_of(mine));
+        const int share = (o.top + warps - 1) / warps;
+        const uint32_t l = __shfl_sync(~0u, sorted, o.top - 1), s = __shfl_sync(~0u, sorted, share - 1);
+        if (lane == 0) sh.largest[warp] = l, sh.share[warp] = s;
+    }
     __syncthreads();
-    p = Part{sh.m[0], sh.s[0], sh.t[0]};
-    for (int w = 1; w < warps; w++) p = join(p, Part{sh.m[w], sh.s[w], sh.t[w]}, c);
+    {   // each warp joins the warps' parts by its lanes
+        p = lane < warps ? sh.part[lane] : empty_part();
+        p = join_lanes(p);
+    }
 
     if (kTop) {
-        const int groups = (v1 - v0 + (1 << shift) - 1) >> shift;
+        const int groups = kOnce ? v1 > v0 : (v1 - v0 + (1 << shift) - 1) >> shift;
         if (p.m != p.m) {
-            search<T, kMask>(src, sh, v0, v1, shift, nullptr, groups, o.top);
+            search<T, kMask>(src, sh, v0, v1, kOnce ? 0 : shift, nullptr, kOnce ? v1 - v0 : groups, o.top);
+        } else if (kOnce) {
+            const uint32_t l = __reduce_max_sync(~0u, lane < warps ? sh.largest[lane] : 0u);
+            const uint32_t s = __reduce_min_sync(~0u, lane < warps ? sh.share[lane] : ~0u);
+            const uint32_t threshold = max(max(l, s), kNothing + 1);
+#pragma unroll
+            for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v0 + warp * kTile + u * 32 + lane, threshold);
+            __syncthreads();
+            const int found = sh.found;
+            if (found <= kFound) rank_entries(sh.entries, found, o.top, sh.list);
+            else search<T, kMask>(src, sh, v0, v1, 0, nullptr, v1 - v0, o.top);
         } else {
             const int chosen = min(o.top, groups);
-            for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+            uint32_t keys[kGroups / 32];
+#pragma unroll
+            for (int i = 0; i < kGroups / 32; i++) keys[i] = sh.group[i * 32 + lane];
+            for (int g = warp; g < groups; g += warps) {
                 const uint32_t key = sh.group[g];
                 int above = 0;
-                for (int k = 0; k < groups; k++) above += sh.group[k] > key || (sh.group[k] == key && k < g);
-                if (above < chosen) sh.order[above] = g;
-                if (above == o.top - 1) sh.threshold = key;
+#pragma unroll
+                for (int i = 0; i < kGroups / 32; i++)
+                    if (i * 32 < groups) above += keys[i] > key || (keys[i] == key && i * 32 + lane < g);
+                above = __reduce_add_sync(~0u, above);
+                if (lane == 0) {
+                    if (above < chosen) sh.order[above] = g;
+                    if (above == o.top - 1) sh.threshold = key;
+                }
             }
             if (groups < o.top && threadIdx.x == 0) sh.threshold = 0;
             __syncthreads();
             const uint32_t threshold = max(sh.threshold, kNothing + 1);
-            for (int i = threadIdx.x; i < chosen << shift; i += blockDim.x) {
-                const int v = v0 + (sh.order[i >> shift] << shift) + (i & ((1 << shift) - 1));
-                if (v >= v1) continue;
-                const uint4 q = src.load(v);
-                if (key_of(most<T>(q)) < threshold) continue;
+            for (int i = threadIdx.x; i < chosen << shift; i += blockDim.x * kUnroll) {
+                int v[kUnroll];
 #pragma unroll
-                for (int n = 0; n < N; n++) {
-                    const uint32_t key = key_of(element<T>(q, n));
-                    if (key < threshold) continue;
-                    const int at = atomicAdd(&sh.found, 1);
-                    if (at < kFound) sh.entries[at] = entry_of(key, v * N - src.head + n);
+                for (int u = 0; u < kUnroll; u++) {
+                    const int k = i + u * blockDim.x;
+                    v[u] = k < chosen << shift ? v0 + (sh.order[k >> shift] << shift) + (k & ((1 << shift) - 1)) : v1;
+                    q[u] = v[u] < v1 ? src.load(v[u]) : no_vector<T>();
                 }
+#pragma unroll
+                for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v[u], threshold);
             }
             __syncthreads();
             const int found = sh.found;
@@ -500,12 +732,14 @@ __global__ void __launch_bounds__(kThreads) long_kernel(Rows a, Out o, int clust
     }
 
     if (cluster > 1) {
-        if (threadIdx.x == 0) sh.part = p;
+        if (threadIdx.x == 0) sh.all = p;
         cluster_sync();
         if (rank == 0) {
-            for (int r = 1; r < cluster; r++)
-                p = join(p, Part{__uint_as_float(remote(&sh.part.m, r)), __uint_as_float(remote(&sh.part.s, r)),
-                                 __uint_as_float(remote(&sh.part.t, r))}, c);
+            p = empty_part();
+            if (lane < cluster)
+                p = Part{remote_float(&sh.all.m, lane), remote_float(&sh.all.r, lane), remote_float(&sh.all.s, lane),
+                         remote_float(&sh.all.t, lane)};
+            p = join_lanes(p);
             if (kTop) {
                 if (threadIdx.x == 0) sh.found = 0;
                 __syncthreads();
@@ -522,14 +756,18 @@ __global__ void __launch_bounds__(kThreads) long_kernel(Rows a, Out o, int clust
         cluster_sync();   // no block leaves while its shared memory is read
         if (rank) return;
     }
-    const Row r(p);
+    const bool far = out_of_range(p);
+    if (far) {
+        const float2 st = far_sums(src, p.m, c, (int)threadIdx.x, (int)blockDim.x);
+        if (lane == 0) sh.far[warp] = st;
+        __syncthreads();
+        p.s = p.t = 0.0f;
+        for (int w = 0; w < warps; w++) p.s += sh.far[w].x, p.t += sh.far[w].y;
+    }
+    const Row r = far ? Row::about_maximum(p) : Row(p, c);
     if (threadIdx.x == 0) write_row<T>(a, o, row, r);
     if (kTop)
-        for (int k = threadIdx.x; k < o.top; k += blockDim.x) {
-            const uint64_t e = sh.list[k];
-            o.top_ids[row * o.top + k] = e ? index_of(e) : -1;
-            o.top_logp[row * o.top + k] = e ? r.logp(of_key((uint32_t)(e >> 32)), a.scale) : -kInf;
-        }
+        for (int k = threadIdx.x; k < o.top; k += blockDim.x) write_top(o, row, k, sh.list[k], r, a.scale);
 }
 static_assert(kMaxCluster * B3X_TRAIN_MAX_TOP <= kFound, "the blocks' alternatives are ranked at once");
 
@@ -542,16 +780,27 @@ int launch_short(const Rows& a, const Out& o, cudaStream_t s) {
 
 template <class T, bool kMask, bool kTop>
 int launch_long(const Rows& a, const Out& o, cudaStream_t s) {
-    const int nv = (int)(((long long)a.width + Vec<T>::n - 1) / Vec<T>::n) + 1;
+    // the most vectors that a row has
+    const bool even = (uintptr_t)a.logits % 16 == 0 && a.row_stride * (long long)sizeof(T) % 16 == 0;
+    const int nv = (int)(((long long)a.width + Vec<T>::n - 1) / Vec<T>::n) + (even ? 0 : 1);
+    if (nv <= 4 * 32) {
+        const unsigned grid = (unsigned)((a.rows + kRowWarps - 1) / kRowWarps);
+        if (nv <= 32) row_kernel<T, kMask, kTop, 1><<<grid, kRowWarps * 32, 0, s>>>(a, o);
+        else if (nv <= 64) row_kernel<T, kMask, kTop, 2><<<grid, kRowWarps * 32, 0, s>>>(a, o);
+        else row_kernel<T, kMask, kTop, 4><<<grid, kRowWarps * 32, 0, s>>>(a, o);
+        return (int)cudaGetLastError();
+    }
     // a cluster a row while rows alone leave SMs idle and each block keeps 512 vectors
     int cluster = 1;
     while (cluster < kMaxCluster && a.rows * cluster * 2 <= 296 && nv / (cluster * 2) >= 512) cluster *= 2;
-    const int each = (nv + cluster - 1) / cluster;
-    int warps = 1;
-    while (warps < kMaxWarps && warps * 32 * kUnroll < each) warps *= 2;
+    int each = (nv + cluster - 1) / cluster;
+    const bool once = each <= kMaxWarps * kTile;
+    const int warps = once ? (each + kTile - 1) / kTile : kMaxWarps;
     int shift = 0;
-    while ((each + (1 << shift) - 1) >> shift > kGroups) shift++;
-    if (shift == 6) shift = 7;
+    if (!once) {
+        shift = each <= 32 * kGroups ? 5 : 7;
+        while ((each + (1 << shift) - 1) >> shift > kGroups) shift++;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * cluster));
     cfg.blockDim = dim3(warps * 32);
@@ -562,7 +811,8 @@ int launch_long(const Rows& a, const Out& o, cudaStream_t s) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, kMaxWarps * 32>, a, o, cluster, shift);
+    if (once) return (int)cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, true>, a, o, cluster, shift);
+    return (int)cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, false>, a, o, cluster, shift);
 }
 
 template <class T>
@@ -571,8 +821,6 @@ int launch(const Rows& a, const Out& o, cudaStream_t s) {
     if (a.width <= kShort * 2) return launch_short<T, 2>(a, o, s);
     if (a.width <= kShort * 4) return launch_short<T, 4>(a, o, s);
     if (a.width <= kShort * 8) return launch_short<T, 8>(a, o, s);
-    if (a.width <= kShort * 16) return launch_short<T, 16>(a, o, s);
-    if (a.width <= kShort * 32) return launch_short<T, 32>(a, o, s);
     if (a.mask) return o.top ? launch_long<T, true, true>(a, o, s) : launch_long<T, true, false>(a, o, s);
     return o.top ? launch_long<T, false, true>(a, o, s) : launch_long<T, false, false>(a, o, s);
 }
