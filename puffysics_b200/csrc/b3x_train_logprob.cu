@@ -403,6 +403,19 @@ __device__ __forceinline__ uint32_t sort_lanes(uint32_t key) {
     return key;
 }
 
+// The 32 largest of two sorted lists, sorted: the larger of each key and its
+// mirror image rise and fall once.
+__device__ __forceinline__ uint32_t merge_lanes(uint32_t key, uint32_t mirrored) {
+    const int lane = threadIdx.x % 32;
+    key = max(key, mirrored);
+#pragma unroll
+    for (int j = 16; j; j /= 2) {
+        const uint32_t other = __shfl_xor_sync(~0u, key, j);
+        key = (lane & j) == 0 ? max(key, other) : min(key, other);
+    }
+    return key;
+}
+
 __device__ __forceinline__ void write_top(const Out& o, long long row, int k, uint64_t e, const Row& r, float scale) {
     o.top_ids[row * o.top + k] = e ? index_of(e) : -1;
     o.top_logp[row * o.top + k] = e ? r.logp(of_key((uint32_t)(e >> 32)), scale) : -kInf;
@@ -509,7 +522,7 @@ __global__ void __launch_bounds__(kRowWarps * 32) row_kernel(Rows a, Out o) {
 // ---- rows of a block or a cluster ------------------------------------------------------------
 constexpr int kUnroll = 4;           // vectors a thread has in flight
 constexpr int kTile = 32 * kUnroll;  // vectors a warp takes at a time
-constexpr int kGroups = 256;         // groups of consecutive vectors whose maxima are kept
+constexpr int kGroups = 512;         // groups of consecutive vectors whose maxima are kept
 constexpr int kFound = 512;          // logits at or above the threshold that are ranked at once
 constexpr int kMaxWarps = 16;
 constexpr int kMaxCluster = 8;
@@ -518,10 +531,9 @@ struct Shared {
     Part part[kMaxWarps];
     Part all;                         // this block's
     uint32_t group[kGroups];
-    int order[B3X_TRAIN_MAX_TOP];
-    uint32_t threshold;
-    uint32_t largest[kMaxWarps], share[kMaxWarps];
-    int found;
+    uint32_t sorted[kMaxWarps][32];   // the lanes' maxima
+    int order[kGroups];
+    int chosen, found;
     uint64_t list[B3X_TRAIN_MAX_TOP]; // this block's alternatives
     uint64_t entries[kFound];
     uint64_t warp_best[kMaxWarps];
@@ -601,16 +613,26 @@ __device__ __forceinline__ void gather(const Source<T, kMask>& src, Shared& sh, 
     }
 }
 
+// The `top` groups with the largest maxima, the first among equal ones: they hold the `top` largest logits.
+__device__ __noinline__ void best_groups(Shared& sh, int groups, int top) {
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+        const uint32_t key = sh.group[g];
+        int above = 0;
+        for (int k = 0; k < groups; k++) above += sh.group[k] > key || (sh.group[k] == key && k < g);
+        if (above < top) sh.order[above] = g;
+    }
+    __syncthreads();
+}
+
 // One block, or one cluster of blocks, a row; the row is read once.  kOnce: each
 // warp has one tile, which stays in its registers.  Otherwise the warps walk
 // over the row with their sums running.
 //
-// Alternatives.  kOnce: a threshold that K logits reach, from the lanes' sorted
-// maxima: the K-th of any warp's, or the least of every warp's (K / warps)-th.
-// Otherwise the maxima of groups of 2^shift consecutive vectors are kept.  The K
-// groups with the largest maxima (the first among equal ones) hold the K largest
-// logits, and the K-th of those maxima is at most the K-th largest logit: those
-// groups are read again, from L2.  What reaches the threshold is ranked.
+// Alternatives.  The lanes' maxima are sorted by warps and merged: the K-th of
+// them is at most the K-th largest logit.  What reaches it is ranked: from the
+// registers, or, where the row was walked over, from the groups of 2^shift
+// consecutive vectors whose maxima (kept beside) reach it, which are read again
+// from L2.
 template <class T, bool kMask, bool kTop, bool kOnce>
 __global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, int cluster, int shift) {
     __shared__ Shared sh;
@@ -625,7 +647,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, 
     if (kTop) {
         if (!kOnce)
             for (int i = threadIdx.x; i < kGroups; i += blockDim.x) sh.group[i] = 0;
-        if (threadIdx.x == 0) sh.found = 0;
+        if (threadIdx.x == 0) sh.found = sh.chosen = 0;
         __syncthreads();
     }
 
@@ -650,7 +672,13 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, 
             if (shift >= 7) {
                 const uint32_t key = __reduce_max_sync(~0u, key_of(here));
                 if (lane == 0) atomicMax(&sh.group[(base - v0) >> shift], key);
-            } else {   // 5: a group is a warp's vectors of one u
+            } else if (shift == 6) {   // a group is a warp's vectors of two u
+#pragma unroll
+                for (int u = 0; u < kUnroll; u += 2) {
+                    const uint32_t key = __reduce_max_sync(~0u, key_of(max_nan(top[u], top[u + 1])));
+                    if (lane == 0 && base + u * 32 < v1) sh.group[(base - v0) / 64 + u / 2] = key;
+                }
+            } else {                   // 5: of one u
 #pragma unroll
                 for (int u = 0; u < kUnroll; u++) {
                     const uint32_t key = __reduce_max_sync(~0u, key_of(top[u]));
@@ -666,11 +694,18 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, 
     const float mine = p.m;
     p = join_lanes(p);
     if (lane == 0) sh.part[warp] = p;
-    if (kTop && kOnce) {
-        const uint32_t sorted = sort_lanes(key_of(mine));
-        const int share = (o.top + warps - 1) / warps;
-        const uint32_t l = __shfl_sync(~0u, sorted, o.top - 1), s = __shfl_sync(~0u, sorted, share - 1);
-        if (lane == 0) sh.largest[warp] = l, sh.share[warp] = s;
+    if (kTop) {
+        uint32_t key = sort_lanes(key_of(mine));
+        sh.sorted[warp][lane] = key;
+        int half = 1;
+        while (half < warps) half *= 2;
+        while (half /= 2) {
+            __syncthreads();
+            if (warp < half && warp + half < warps) {
+                key = merge_lanes(key, sh.sorted[warp + half][31 - lane]);
+                sh.sorted[warp][lane] = key;
+            }
+        }
     }
     __syncthreads();
     {   // each warp joins the warps' parts by its lanes
@@ -679,54 +714,41 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, 
     }
 
     if (kTop) {
-        const int groups = kOnce ? v1 > v0 : (v1 - v0 + (1 << shift) - 1) >> shift;
+        const int groups = (v1 - v0 + (1 << shift) - 1) >> shift;
+        const uint32_t threshold = max(sh.sorted[0][o.top - 1], kNothing + 1);
         if (p.m != p.m) {
-            search<T, kMask>(src, sh, v0, v1, kOnce ? 0 : shift, nullptr, kOnce ? v1 - v0 : groups, o.top);
-        } else if (kOnce) {
-            const uint32_t l = __reduce_max_sync(~0u, lane < warps ? sh.largest[lane] : 0u);
-            const uint32_t s = __reduce_min_sync(~0u, lane < warps ? sh.share[lane] : ~0u);
-            const uint32_t threshold = max(max(l, s), kNothing + 1);
-#pragma unroll
-            for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v0 + warp * kTile + u * 32 + lane, threshold);
-            __syncthreads();
-            const int found = sh.found;
-            if (found <= kFound) rank_entries(sh.entries, found, o.top, sh.list);
-            else search<T, kMask>(src, sh, v0, v1, 0, nullptr, v1 - v0, o.top);
+            search<T, kMask>(src, sh, v0, v1, shift, nullptr, groups, o.top);
         } else {
-            const int chosen = min(o.top, groups);
-            uint32_t keys[kGroups / 32];
+            if (kOnce) {
 #pragma unroll
-            for (int i = 0; i < kGroups / 32; i++) keys[i] = sh.group[i * 32 + lane];
-            for (int g = warp; g < groups; g += warps) {
-                const uint32_t key = sh.group[g];
-                int above = 0;
+                for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v0 + warp * kTile + u * 32 + lane, threshold);
+            } else {
+                for (int g = threadIdx.x; g < groups; g += blockDim.x)
+                    if (sh.group[g] >= threshold) sh.order[atomicAdd(&sh.chosen, 1)] = g;
+                __syncthreads();
+                const int again = sh.chosen << shift;
+                for (int i = threadIdx.x; i < again; i += blockDim.x * kUnroll) {
+                    int v[kUnroll];
 #pragma unroll
-                for (int i = 0; i < kGroups / 32; i++)
-                    if (i * 32 < groups) above += keys[i] > key || (keys[i] == key && i * 32 + lane < g);
-                above = __reduce_add_sync(~0u, above);
-                if (lane == 0) {
-                    if (above < chosen) sh.order[above] = g;
-                    if (above == o.top - 1) sh.threshold = key;
+                    for (int u = 0; u < kUnroll; u++) {
+                        const int k = i + u * blockDim.x;
+                        v[u] = k < again ? v0 + (sh.order[k >> shift] << shift) + (k & ((1 << shift) - 1)) : v1;
+                        q[u] = v[u] < v1 ? src.load(v[u]) : no_vector<T>();
+                    }
+#pragma unroll
+                    for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v[u], threshold);
                 }
-            }
-            if (groups < o.top && threadIdx.x == 0) sh.threshold = 0;
-            __syncthreads();
-            const uint32_t threshold = max(sh.threshold, kNothing + 1);
-            for (int i = threadIdx.x; i < chosen << shift; i += blockDim.x * kUnroll) {
-                int v[kUnroll];
-#pragma unroll
-                for (int u = 0; u < kUnroll; u++) {
-                    const int k = i + u * blockDim.x;
-                    v[u] = k < chosen << shift ? v0 + (sh.order[k >> shift] << shift) + (k & ((1 << shift) - 1)) : v1;
-                    q[u] = v[u] < v1 ? src.load(v[u]) : no_vector<T>();
-                }
-#pragma unroll
-                for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v[u], threshold);
             }
             __syncthreads();
             const int found = sh.found;
-            if (found <= kFound) rank_entries(sh.entries, found, o.top, sh.list);
-            else search<T, kMask>(src, sh, v0, v1, shift, sh.order, chosen, o.top);
+            if (found <= kFound) {
+                rank_entries(sh.entries, found, o.top, sh.list);
+            } else if (kOnce) {
+                search<T, kMask>(src, sh, v0, v1, 0, nullptr, v1 - v0, o.top);
+            } else {
+                best_groups(sh, groups, o.top);
+                search<T, kMask>(src, sh, v0, v1, shift, sh.order, min(o.top, groups), o.top);
+            }
         }
         __syncthreads();
     }
@@ -794,11 +816,15 @@ int launch_long(const Rows& a, const Out& o, cudaStream_t s) {
     int cluster = 1;
     while (cluster < kMaxCluster && a.rows * cluster * 2 <= 296 && nv / (cluster * 2) >= 512) cluster *= 2;
     int each = (nv + cluster - 1) / cluster;
-    const bool once = each <= kMaxWarps * kTile;
-    const int warps = once ? (each + kTile - 1) / kTile : kMaxWarps;
+    // Rows for every SM several times over: small blocks, whose ends overlap (4,096 rows of 131,072 bf16 with 20
+    // alternatives 254 us with 16 warps, 221 with 4; 2,048 masked rows of 50,001 120 us with 16, 75 with 2).  Fewer:
+    // 16 warps (128 rows of 131,072 17 us, with 4 warps 24).
+    const bool many = a.rows * cluster >= 592;
+    const bool once = each <= (many ? 4 : kMaxWarps) * kTile;
+    const int warps = once ? (each + kTile - 1) / kTile : !many ? kMaxWarps : each > 8192 ? 4 : 2;
     int shift = 0;
     if (!once) {
-        shift = each <= 32 * kGroups ? 5 : 7;
+        shift = each <= 8192 ? 5 : 6;   // some hundred groups
         while ((each + (1 << shift) - 1) >> shift > kGroups) shift++;
     }
     cudaLaunchConfig_t cfg = {};
