@@ -1,5 +1,15 @@
 // b3x_train_advantage.cu -- generalised advantages and returns of a rollout
 // (b3x_train.h).
+//
+// A_t = x_t + a_t A_{t+1} with x_t = delta_t and a_t = gamma lam, or 0 where the
+// step ends an episode or is an environment's last.  Steps in a row compose to
+// a pair (a, b) too, A = b + a A_after, and pairs compose associatively; so time
+// is split over threads: each composes a few consecutive steps in registers, a
+// suffix scan over lanes, warps and blocks gives each thread the A after its
+// steps, and it walks back through them.  Inputs are read once and outputs
+// written once; bound by memory for large rollouts and by the launch and one
+// trip to memory for those of an environment batch.  Where a is 0 nothing is
+// multiplied: what lies beyond a terminal may be NaN.
 #include <cmath>
 
 #include "b3x_train_common.cuh"
@@ -16,37 +26,291 @@ struct Rollout {
     float *advantages, *returns;
     long long rt, rn, vt, vn, dt, dn, ln, at, an, ot, on;
     float gamma, decay;  // gamma, gamma * lam
-    int terminal_bytes;
 };
 
-__device__ __forceinline__ bool terminal(const Rollout& a, long long i) {
-    return a.terminal_bytes == 4 ? ((const float*)a.terminals)[i] != 0.0f : ((const unsigned char*)a.terminals)[i] != 0;
+// A = b + a A_after.
+struct Pair {
+    float a, b;
+};
+__device__ __forceinline__ float apply(Pair p, float after) { return p.a != 0.0f ? __fmaf_rn(p.a, after, p.b) : p.b; }
+__device__ __forceinline__ Pair compose(Pair first, Pair then) { return Pair{first.a * then.a, apply(first, then.b)}; }
+
+// kSteps consecutive steps of one environment.
+template <int kSteps>
+struct Steps {
+    float x[kSteps], v[kSteps];
+    unsigned on;      // bit i: a of step i is gamma lam
+    unsigned in;      // bit i: the step is one of the range's
+    unsigned real;    // bit i: and before the environment's end
+
+    __device__ __forceinline__ Pair pair(float decay) const {
+        Pair p{1.0f, 0.0f};
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; i--)
+            if (in >> i & 1) p = on >> i & 1 ? Pair{decay * p.a, __fmaf_rn(decay, p.b, x[i])} : Pair{0.0f, x[i]};
+        return p;
+    }
+};
+
+template <class V> __device__ __forceinline__ float4 load4(const V* p);
+template <> __device__ __forceinline__ float4 load4(const float* p) { return __ldcs(reinterpret_cast<const float4*>(p)); }
+template <> __device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
+    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(p));
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16),
+                       __uint_as_float(w.y & 0xFFFF0000u));
+}
+template <> __device__ __forceinline__ float4 load4(const __half* p) {
+    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(p));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+template <> __device__ __forceinline__ float4 load4(const unsigned char* p) {
+    const unsigned w = __ldcs(reinterpret_cast<const unsigned*>(p));
+    return make_float4((float)(w & 0xFF), (float)(w >> 8 & 0xFF), (float)(w >> 16 & 0xFF), (float)(w >> 24));
 }
 
-// One thread an environment, from its last step to its first.
-template <class V>
-__global__ void __launch_bounds__(128) advantage_kernel(Rollout a) {
-    const long long n = (long long)blockIdx.x * 128 + threadIdx.x;
-    if (n >= a.envs) return;
-    long long len = a.lengths ? a.lengths[n] : a.steps;
-    len = len < 0 ? 0 : len > a.steps ? a.steps : len;
-    for (long long t = a.steps - 1; t >= len; t--) {
-        a.advantages[t * a.at + n * a.an] = 0.0f;
-        if (a.returns) a.returns[t * a.ot + n * a.on] = 0.0f;
+// Steps [t, t + kSteps) of environment n, those in [t0, t1).  kVec: time is
+// consecutive in memory and t is on a 4-element boundary of every array.
+template <class V, class D, int kSteps, bool kVec>
+__device__ __forceinline__ Steps<kSteps> load_steps(const Rollout& a, long long n, long long t, long long t0, long long t1,
+                                                    long long len) {
+    Steps<kSteps> s;
+    const float* r = a.rewards + n * a.rn;
+    const V* v = (const V*)a.values + n * a.vn;
+    const D* d = (const D*)a.terminals + n * a.dn;
+    float rew[kSteps];
+    bool end[kSteps];
+    s.on = s.in = s.real = 0;
+    if (kVec && t >= t0 && t + kSteps <= t1 && t + kSteps <= len) {
+#pragma unroll
+        for (int i = 0; i < kSteps; i += 4) {
+            const float4 x = load4(r + t + i), y = load4(v + t + i), z = load4(d + t + i);
+            rew[i] = x.x, rew[i + 1] = x.y, rew[i + 2] = x.z, rew[i + 3] = x.w;
+            s.v[i] = y.x, s.v[i + 1] = y.y, s.v[i + 2] = y.z, s.v[i + 3] = y.w;
+            end[i] = z.x != 0.0f, end[i + 1] = z.y != 0.0f, end[i + 2] = z.z != 0.0f, end[i + 3] = z.w != 0.0f;
+        }
+        s.in = s.real = (1u << kSteps) - 1;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; i++) {
+            const long long k = t + i;
+            const bool in = k >= t0 && k < t1, real = in && k < len;
+            rew[i] = s.v[i] = 0.0f;
+            end[i] = true;
+            if (real) {
+                rew[i] = __ldcs(r + k * a.rt);
+                s.v[i] = to_float(v[k * a.vt]);
+                end[i] = d[k * a.dt] != (D)0;
+            }
+            s.in |= in ? 1u << i : 0;
+            s.real |= real ? 1u << i : 0;
+        }
     }
-    float after = len ? to_float(((const V*)a.last_values)[n * a.ln]) : 0.0f, ahead = 0.0f;
-    for (long long t = len - 1; t >= 0; t--) {
-        const float v = to_float(((const V*)a.values)[t * a.vt + n * a.vn]);
-        const bool end = terminal(a, t * a.dt + n * a.dn);
-        float x = a.rewards[t * a.rt + n * a.rn];
-        if (!end) x += a.gamma * after;
-        x -= v;
-        if (!end) x += a.decay * ahead;
-        ahead = x;
-        after = v;
-        a.advantages[t * a.at + n * a.an] = ahead;
-        if (a.returns) a.returns[t * a.ot + n * a.on] = ahead + v;
+    // the value after the last of them
+    float after = 0.0f;
+    const long long k = t + kSteps;
+    if (s.real) {
+        if (k < len) after = to_float(v[k * a.vt]);
+        else after = to_float(((const V*)a.last_values)[n * a.ln]);
     }
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; i--) {
+        const bool real = s.real >> i & 1;
+        const float next = i == kSteps - 1 ? after : (s.real >> (i + 1) & 1) ? s.v[i + 1] : after;
+        s.x[i] = real ? (end[i] ? rew[i] : __fmaf_rn(a.gamma, next, rew[i])) - s.v[i] : 0.0f;
+        s.on |= real && !end[i] && t + i != len - 1 && a.decay != 0.0f ? 1u << i : 0;
+    }
+    return s;
+}
+
+template <int kSteps, bool kVec>
+__device__ __forceinline__ void store_steps(const Rollout& a, const Steps<kSteps>& s, long long n, long long t, float after) {
+    float A[kSteps];
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; i--) {
+        if (s.in >> i & 1) after = s.on >> i & 1 ? __fmaf_rn(a.decay, after, s.x[i]) : s.x[i];
+        A[i] = after;
+    }
+    float* adv = a.advantages + n * a.an;
+    float* ret = a.returns ? a.returns + n * a.on : nullptr;
+    if (kVec && s.real == (1u << kSteps) - 1) {
+#pragma unroll
+        for (int i = 0; i < kSteps; i += 4) {
+            __stcs(reinterpret_cast<float4*>(adv + t + i), make_float4(A[i], A[i + 1], A[i + 2], A[i + 3]));
+            if (ret)
+                __stcs(reinterpret_cast<float4*>(ret + t + i),
+                       make_float4(A[i] + s.v[i], A[i + 1] + s.v[i + 1], A[i + 2] + s.v[i + 2], A[i + 3] + s.v[i + 3]));
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+        if (!(s.in >> i & 1)) continue;
+        const bool real = s.real >> i & 1;
+        adv[(t + i) * a.at] = real ? A[i] : 0.0f;
+        if (ret) ret[(t + i) * a.ot] = real ? A[i] + s.v[i] : 0.0f;
+    }
+}
+
+__device__ __forceinline__ long long length_of(const Rollout& a, long long n) {
+    const long long len = a.lengths ? a.lengths[n] : a.steps;
+    return len < 0 ? 0 : len > a.steps ? a.steps : len;
+}
+
+// Steps before the first whole group of 4 in memory.
+__device__ __forceinline__ int lead_of(const Rollout& a, long long n) { return (int)((uintptr_t)(a.rewards + n * a.rn) / 4 % 4); }
+
+// Lanes `apart` from one another hold consecutive steps: composes each with all after it within `width` lanes.
+__device__ __forceinline__ Pair scan_lanes(Pair p, int apart, int width) {
+    const int lane = threadIdx.x % width;
+    for (int o = apart; o < width; o *= 2) {
+        const Pair then{__shfl_down_sync(~0u, p.a, o, width), __shfl_down_sync(~0u, p.b, o, width)};
+        if (lane + o < width) p = compose(p, then);
+    }
+    return p;
+}
+
+// Many environments, time consecutive in memory: `group` lanes an environment,
+// 4 steps a lane, from the last steps to the first.
+constexpr int kRowThreads = 256;
+
+template <class V, class D>
+__global__ void __launch_bounds__(kRowThreads) advantage_rows_kernel(const Rollout a, int group) {
+    const long long n = ((long long)blockIdx.x * kRowThreads + threadIdx.x) / group;
+    const int lane = threadIdx.x % group;
+    const bool on = n < a.envs;
+    const long long len = on ? length_of(a, n) : 0;
+    const int lead = on ? lead_of(a, n) : 0;
+    const long long steps = on ? a.steps : 0;
+    // the same number of turns for a warp's environments
+    const long long turns = (a.steps + 3 + 4ll * group - 1) / (4ll * group);
+    float carry = 0.0f;
+    for (long long k = turns - 1; k >= 0; k--) {
+        const long long t = (k * group + lane) * 4 - lead;
+        const Steps<4> s = load_steps<V, D, 4, true>(a, n, t, 0, steps, len);
+        const Pair p = scan_lanes(s.pair(a.decay), 1, group);
+        const Pair then{__shfl_down_sync(~0u, p.a, 1, group), __shfl_down_sync(~0u, p.b, 1, group)};
+        if (on) store_steps<4, true>(a, s, n, t, lane == group - 1 ? carry : apply(then, carry));
+        const Pair all{__shfl_sync(~0u, p.a, 0, group), __shfl_sync(~0u, p.b, 0, group)};
+        carry = apply(all, carry);
+    }
+}
+
+__device__ __forceinline__ unsigned cluster_rank() {
+    unsigned r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
+}
+__device__ __forceinline__ float remote_float(const void* p, unsigned rank) {
+    unsigned at;
+    float w;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(at) : "memory");
+    return w;
+}
+
+constexpr int kMaxThreads = 1024;
+constexpr int kMaxCluster = 8;
+
+struct Shared {
+    Pair total[2][kMaxThreads / 32][32];   // each warp's steps, by environment
+    Pair block[32];                        // the block's
+};
+
+// 2^env_bits environments a block, neighbouring lanes neighbouring environments,
+// kSteps steps a thread; a cluster's blocks divide the time.  Long times take
+// several turns of the block, from the last steps to the first, each with what
+// the one before carried; the blocks of a cluster go through their part once
+// before, for its pair alone (their second reading comes from L2).
+template <class V, class D, int kSteps, bool kVec>
+__global__ void __launch_bounds__(kMaxThreads) advantage_kernel(const Rollout a, int env_bits, int cluster) {
+    __shared__ Shared sh;
+    const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int nx = 1 << env_bits, e = threadIdx.x & (nx - 1), seg = threadIdx.x >> env_bits;
+    const int rank = cluster > 1 ? (int)cluster_rank() : 0;
+    const long long n = (long long)(blockIdx.x / cluster) * nx + e;
+    const bool on = n < a.envs;
+    const long long len = on ? length_of(a, n) : 0;
+    const int lead = kVec ? lead_of(a, n < a.envs ? n : a.envs - 1) : 0;
+    const long long turn = (long long)(blockDim.x >> env_bits) * kSteps;   // steps of a turn
+    // this block's part of the time, from -lead on, in whole turns
+    const long long turns = (a.steps + lead + turn - 1) / turn, each = (turns + cluster - 1) / cluster;
+    const long long k0 = min(turns, each * rank), k1 = min(turns, k0 + each);
+    const long long t1 = on ? a.steps : 0;
+
+    int buffer = 0;
+    Pair carry{1.0f, 0.0f};
+    for (int phase = cluster > 1 ? 0 : 1; phase < 2; phase++) {
+        for (long long k = k1 - 1; k >= k0; k--) {
+            const long long t = k * turn + (long long)seg * kSteps - lead;
+            const Steps<kSteps> s = load_steps<V, D, kSteps, kVec>(a, n, t, 0, t1, len);
+            const Pair p = scan_lanes(s.pair(a.decay), nx, 32);
+            if (lane < nx) sh.total[buffer][warp][lane] = p;
+            __syncthreads();
+            Pair here = carry;
+            for (int w = warps - 1; w >= 0; w--) {
+                if (w == warp) here = carry;
+                carry = compose(sh.total[buffer][w][e], carry);
+            }
+            buffer ^= 1;
+            if (phase == 0) continue;
+            const Pair then{__shfl_down_sync(~0u, p.a, nx & 31), __shfl_down_sync(~0u, p.b, nx & 31)};
+            if (on) store_steps<kSteps, kVec>(a, s, n, t, lane + nx >= 32 ? here.b : apply(then, here.b));
+        }
+        if (phase == 0) {
+            if (threadIdx.x < nx) sh.block[threadIdx.x] = carry;
+            cluster_sync();
+            Pair after{1.0f, 0.0f};
+            for (int r = cluster - 1; r > rank; r--)
+                after = compose(Pair{remote_float(&sh.block[e].a, r), remote_float(&sh.block[e].b, r)}, after);
+            carry = after;
+            cluster_sync();   // no block leaves, or writes there, while another reads
+        }
+    }
+}
+
+template <class V, class D>
+int launch(const Rollout& a, bool vec, cudaStream_t s) {
+    // many environments: lanes for each of them (none to wait for); 4 steps a lane
+    if (vec && (a.steps <= 128 || a.envs >= 4096)) {
+        int group = 1;
+        while (group < 32 && group * 4 < a.steps + 3) group *= 2;
+        const long long blocks = (a.envs * group + kRowThreads - 1) / kRowThreads;
+        if (blocks > 0x7fffffff) return (int)cudaErrorInvalidValue;
+        advantage_rows_kernel<V, D><<<(unsigned)blocks, kRowThreads, 0, s>>>(a, group);
+        return (int)cudaGetLastError();
+    }
+    const int steps = vec ? 4 : 8;
+    const long long need = a.steps + (vec ? 3 : 0);
+    // environments side by side where they are neighbours in memory, fewer while that leaves SMs idle or takes turns
+    int bits = 0;
+    if (!vec && (a.rt != 1 || a.steps == 1 || a.rn < a.rt)) {
+        while (bits < 5 && (1 << bits) < a.envs) bits++;
+        while (bits > 0 && ((a.envs + (1 << bits) - 1) >> bits) < 148 && a.steps > ((long long)kMaxThreads >> bits) * steps) bits--;
+    }
+    const long long groups = (a.envs + (1 << bits) - 1) >> bits;
+    // threads for all steps, up to 512 (1024 where blocks are few), then blocks
+    const int most = groups < 148 ? kMaxThreads : 512;
+    int threads = 32;
+    while (threads < most && (long long)(threads >> bits) * steps < need) threads *= 2;
+    int cluster = 1;
+    while (cluster < kMaxCluster && groups * cluster * 2 <= 148 && (long long)(threads >> bits) * steps * cluster < need)
+        cluster *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(groups * cluster));
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    if (vec) return (int)cudaLaunchKernelEx(&cfg, advantage_kernel<V, D, 4, true>, a, bits, cluster);
+    return (int)cudaLaunchKernelEx(&cfg, advantage_kernel<V, D, 8, false>, a, bits, cluster);
 }
 
 }  // namespace
@@ -71,10 +335,20 @@ int b3x_train_advantage_gpu(long long steps, long long envs, const float* reward
         return (int)cudaErrorInvalidValue;
     const Rollout a{steps, envs, rewards, values, terminals, last_values, lengths, advantages, returns,
                     strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6],
-                    strides[7], strides[8], strides[9], strides[10], gamma, gamma * lam, tb};
-    const unsigned grid = (unsigned)((envs + 127) / 128);
-    if (value_type == B3X_F32) advantage_kernel<float><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-    if (value_type == B3X_BF16) advantage_kernel<__nv_bfloat16><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-    if (value_type == B3X_F16) advantage_kernel<__half><<<grid, 128, 0, (cudaStream_t)stream>>>(a);
-    return (int)cudaGetLastError();
+                    strides[7], strides[8], strides[9], strides[10], gamma, gamma * lam};
+    // 4 steps at a time: consecutive in memory, every array's rows at the same place among groups of 4
+    const auto place = [](const void* p, int bytes) { return (uintptr_t)p / bytes % 4; };
+    bool vec = steps > 1 && strides[0] == 1 && strides[2] == 1 && strides[4] == 1 && strides[7] == 1 &&
+               (!returns || strides[9] == 1) && place(values, vb) == place(rewards, 4) &&
+               place(terminals, tb) == place(rewards, 4) && place(advantages, 4) == place(rewards, 4) &&
+               (!returns || place(returns, 4) == place(rewards, 4));
+    if (envs > 1)
+        for (const int i : {3, 5, 8, 10})
+            vec = vec && ((!returns && i == 10) || (strides[i] - strides[1]) % 4 == 0);
+    const cudaStream_t s = (cudaStream_t)stream;
+    const bool f = terminal_type == B3X_F32;
+    if (value_type == B3X_F32) return f ? launch<float, float>(a, vec, s) : launch<float, unsigned char>(a, vec, s);
+    if (value_type == B3X_BF16)
+        return f ? launch<__nv_bfloat16, float>(a, vec, s) : launch<__nv_bfloat16, unsigned char>(a, vec, s);
+    return f ? launch<__half, float>(a, vec, s) : launch<__half, unsigned char>(a, vec, s);
 }
