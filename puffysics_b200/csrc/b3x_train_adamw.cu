@@ -9,10 +9,10 @@ using namespace b3t;
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kChunk = kThreads * 8;    // elements a block takes at a time; a multiple of B3X_TRAIN_BLOCK
-constexpr int kList = 256;              // tensors of one launch: the table travels in the kernel's parameters
+constexpr int kTurn = kThreads * 8;     // elements a block takes at a time: a scale's 256 for each warp
 constexpr int kNormBlocks = 592;        // partial sums of the norm
-static_assert(kChunk % B3X_TRAIN_BLOCK == 0, "a scale's elements stay in one block");
+constexpr int kFew = 16, kMany = 256;   // tensors of one launch: their table travels in the kernel's parameters
+static_assert(B3X_TRAIN_BLOCK == 256, "a warp's 8 elements a lane share a scale");
 
 struct Tensor {
     void* p;
@@ -23,11 +23,12 @@ struct Tensor {
     long long n;
     float keep;          // 1 - lr weight_decay
     unsigned key;        // the tensor's part of the rounding hash
+    int even;            // every array starts at a multiple of 4 elements
 };
 
 template <int N>
 struct List {
-    int count;
+    int count, turns;        // turns of a chunk
     unsigned first[N + 1];   // first chunk of each tensor
     Tensor t[N];
 };
@@ -57,125 +58,313 @@ __host__ __device__ __forceinline__ unsigned mix(unsigned x) {
     return x ^ (x >> 16);
 }
 
-// e4m3 codes of x / scale.  Scaled by 2^-120 the format's exponents are
-// float's, subnormals included, so the code is the upper bits of the word; what
-// is added to the 20 bits below it rounds.
+// Four consecutive elements.
+template <class T> __device__ __forceinline__ void load4(float (&x)[4], const T* p);
+template <> __device__ __forceinline__ void load4(float (&x)[4], const float* p) {
+    const float4 w = __ldcs(reinterpret_cast<const float4*>(p));
+    x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+}
+template <> __device__ __forceinline__ void load4(float (&x)[4], const __nv_bfloat16* p) {
+    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(p));
+    x[0] = __uint_as_float(w.x << 16), x[1] = __uint_as_float(w.x & 0xFFFF0000u);
+    x[2] = __uint_as_float(w.y << 16), x[3] = __uint_as_float(w.y & 0xFFFF0000u);
+}
+template <> __device__ __forceinline__ void load4(float (&x)[4], const __half* p) {
+    const uint2 w = __ldcs(reinterpret_cast<const uint2*>(p));
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+__device__ __forceinline__ void store4(float* p, const float (&x)[4]) {
+    __stcs(reinterpret_cast<float4*>(p), make_float4(x[0], x[1], x[2], x[3]));
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&x)[4]) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(*reinterpret_cast<const unsigned*>(&a), *reinterpret_cast<const unsigned*>(&b)));
+}
+
+// Two e4m3 codes' values.
+__device__ __forceinline__ float2 decode2(unsigned codes) {
+    unsigned h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)codes));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// The e4m3 code of y.  Scaled by 2^-120 the format's exponents are float's,
+// subnormals included, so the code is the upper bits of the word; what is added
+// to the 20 bits below it rounds: random bits up or down in proportion, a half
+// to nearest.
 __device__ __forceinline__ unsigned encode(float y, bool stochastic, unsigned bits16) {
     unsigned w = __float_as_uint(fabsf(y) * 0x1p-120f);
     w += stochastic ? (bits16 << 4 | 8u) : 0x7FFFFu + ((w >> 20) & 1u);
-    w = min(w >> 20, 0x7Eu);
-    return y < 0.0f ? w | 0x80u : w;
+    return min(w >> 20, 0x7Eu) | (y < 0.0f ? 0x80u : 0u);
 }
 
-__device__ __forceinline__ float decode(unsigned code) {
-    const float y = __uint_as_float((code & 0x7Fu) << 20) * 0x1p120f;
-    return code & 0x80u ? -y : y;
+__device__ __forceinline__ float reciprocal(float x) {   // 1 ulp
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
+// The largest of a warp's numbers that are not negative; NaN is the largest.
 __device__ __forceinline__ float warp_most(float x) {
-    for (int o = 16; o; o >>= 1) x = max_nan(x, __shfl_xor_sync(~0u, x, o));
-    return x;
+    return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(x) & 0x7FFFFFFFu));
 }
 
-// A warp takes the elements of one scale at a time, eight apart by 32 for each
-// lane; every operation rounds by itself (the plain formula's bits).
+// A warp takes the 256 elements of one scale at a time, two runs of four a lane,
+// so that every load and store is a whole line however wide its type.  The
+// moments' operations round one by one: their codes are those of the plain
+// formula, bit for bit.
 template <class P, class G, bool kF8, int N>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ List<N> list, const Hyper h,
                                                          const int stochastic) {
     const float gs = h.grad_scale ? *h.grad_scale : 1.0f;
     if (!(fabsf(gs) < kInf)) return;
-    const Tensor& t = list.t[find(list, blockIdx.x)];
-    const unsigned chunk = blockIdx.x - list.first[&t - list.t];
+    const int which = find(list, blockIdx.x);
+    const Tensor& t = list.t[which];
     const int lane = threadIdx.x % 32;
-    const long long base = (long long)chunk * kChunk + threadIdx.x / 32 * B3X_TRAIN_BLOCK;
-    if (base >= t.n) return;
-    float m[8], r[8];
-    float sm = 1.0f, sr = 1.0f;
-    if (kF8) sm = t.scales[base / B3X_TRAIN_BLOCK * 2], sr = t.scales[base / B3X_TRAIN_BLOCK * 2 + 1];
-    float most_m = 0.0f, most_r = 0.0f;
-    for (int k = 0; k < 8; k++) {
-        const long long i = base + k * 32 + lane;
-        m[k] = r[k] = 0.0f;
-        if (i >= t.n) continue;
-        const float g = to_float(((const G*)t.g)[i]) * gs;
-        float v;
+    long long base = ((long long)(blockIdx.x - list.first[which]) * list.turns * (kTurn / 256) + threadIdx.x / 32) * 256;
+    const long long n = t.n;
+    P* const pp = (P*)t.p;
+    const G* const pg = (const G*)t.g;
+    for (int turn = 0; turn < list.turns && base < n; turn++, base += kTurn) {
+        const bool whole = t.even && base + 256 <= n;
+        float p[2][4], g[2][4], m[2][4], v[2][4];
+        uint32_t cm[2], cv[2];
+        float sm = 0.0f, sr = 0.0f;
         if (kF8) {
-            m[k] = decode(((unsigned char*)t.m)[i]) * sm;
-            v = decode(((unsigned char*)t.v)[i]) * sr;
-            v = v * v;
+            const float2 s = *reinterpret_cast<const float2*>(t.scales + base / 256 * 2);
+            sm = s.x, sr = s.y;
+        }
+        if (whole) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const long long i = base + k * 128 + lane * 4;
+                load4(g[k], pg + i);
+                load4(p[k], pp + i);
+                if (kF8) {
+                    cm[k] = __ldcs(reinterpret_cast<const uint32_t*>((const unsigned char*)t.m + i));
+                    cv[k] = __ldcs(reinterpret_cast<const uint32_t*>((const unsigned char*)t.v + i));
+                } else {
+                    load4(m[k], (const float*)t.m + i);
+                    load4(v[k], (const float*)t.v + i);
+                }
+            }
         } else {
-            m[k] = ((float*)t.m)[i];
-            v = ((float*)t.v)[i];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                cm[k] = cv[k] = 0;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const long long i = base + k * 128 + lane * 4 + j;
+                    const bool in = i < n;
+                    g[k][j] = in ? to_float(pg[i]) : 0.0f;
+                    p[k][j] = in ? to_float(pp[i]) : 0.0f;
+                    if (kF8) {
+                        cm[k] |= in ? (uint32_t)((const unsigned char*)t.m)[i] << j * 8 : 0u;
+                        cv[k] |= in ? (uint32_t)((const unsigned char*)t.v)[i] << j * 8 : 0u;
+                    } else {
+                        m[k][j] = in ? ((const float*)t.m)[i] : 0.0f;
+                        v[k][j] = in ? ((const float*)t.v)[i] : 0.0f;
+                    }
+                }
+            }
         }
-        m[k] = m[k] * h.b1 + g * h.c1;
-        v = v * h.b2 + (g * g) * h.c2;
-        r[k] = sqrtf(v);
-        if (!kF8) ((float*)t.m)[i] = m[k], ((float*)t.v)[i] = v;
-        float p = to_float(((P*)t.p)[i]) * t.keep - (m[k] / (r[k] * h.root + h.eps)) * h.rate;
-        if (t.copy) t.copy[i] = __float2bfloat16_rn(p);
-        if (sizeof(P) == 2 && stochastic && fabsf(p) < kInf) {
-            const unsigned low = mix(mix((unsigned)i * 0x9E3779B1u + (unsigned)(i >> 32) * 0x6A09E667u + t.key) + 0x9E3779B1u);
-            p = __uint_as_float((__float_as_uint(p) + (low & 0xFFFFu)) & 0xFFFF0000u);
+        float most_m = 0.0f, most_r = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            if (kF8) {
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    const float2 a = decode2(cm[k] >> j * 8), b = decode2(cv[k] >> j * 8);
+                    m[k][j] = a.x * sm, m[k][j + 1] = a.y * sm;
+                    const float r0 = b.x * sr, r1 = b.y * sr;
+                    v[k][j] = r0 * r0, v[k][j + 1] = r1 * r1;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float x = g[k][j] * gs;
+                m[k][j] = m[k][j] * h.b1 + x * h.c1;
+                v[k][j] = v[k][j] * h.b2 + (x * x) * h.c2;
+                const float r = sqrtf(v[k][j]);
+                p[k][j] = p[k][j] * t.keep - (m[k][j] * reciprocal(r * h.root + h.eps)) * h.rate;
+                if (kF8) {
+                    most_m = max_nan(most_m, fabsf(m[k][j])), most_r = max_nan(most_r, r);
+                    v[k][j] = r;
+                }
+            }
         }
-        ((P*)t.p)[i] = from_float<P>(p);
-        most_m = max_nan(most_m, fabsf(m[k]));
-        most_r = max_nan(most_r, r[k]);
-    }
-    if (!kF8) return;
-    most_m = warp_most(most_m), most_r = warp_most(most_r);
-    const bool zm = most_m < 0x1p-100f, zr = most_r < 0x1p-100f;   // false for NaN
-    const float im = zm ? 0.0f : 448.0f / most_m, ir = zr ? 0.0f : 448.0f / most_r;
-    if (lane == 0) {
-        t.scales[base / B3X_TRAIN_BLOCK * 2] = zm ? 0.0f : most_m / 448.0f;
-        t.scales[base / B3X_TRAIN_BLOCK * 2 + 1] = zr ? 0.0f : most_r / 448.0f;
-    }
-    for (int k = 0; k < 8; k++) {
-        const long long i = base + k * 32 + lane;
-        if (i >= t.n) break;
-        const unsigned bits = mix((unsigned)i * 0x9E3779B1u + (unsigned)(i >> 32) * 0x6A09E667u + t.key);
-        ((unsigned char*)t.m)[i] = (unsigned char)encode(m[k] * im, stochastic, bits & 0xFFFFu);
-        unsigned c = encode(r[k] * ir, stochastic, bits >> 16);
-        if (c == 0 && r[k] > 0.0f && !zr) c = 1;
-        ((unsigned char*)t.v)[i] = (unsigned char)c;
+        if (!kF8) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const long long i = base + k * 128 + lane * 4;
+                if (whole) {
+                    store4((float*)t.m + i, m[k]);
+                    store4((float*)t.v + i, v[k]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (i + j < n) ((float*)t.m)[i + j] = m[k][j], ((float*)t.v)[i + j] = v[k][j];
+                }
+            }
+        }
+        if (t.copy) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const long long i = base + k * 128 + lane * 4;
+                if (whole) {
+                    store4(t.copy + i, p[k]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (i + j < n) t.copy[i + j] = __float2bfloat16_rn(p[k][j]);
+                }
+            }
+        }
+        uint32_t bits[2][4];
+        if (stochastic && (kF8 || sizeof(P) == 2)) {
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const long long i = base + k * 128 + lane * 4 + j;
+                    bits[k][j] = mix((unsigned)i * 0x9E3779B1u + (unsigned)(i >> 32) * 0x6A09E667u + t.key);
+                    if (sizeof(P) == 2 && fabsf(p[k][j]) < kInf) {
+                        const unsigned low = mix(bits[k][j] + 0x9E3779B1u);
+                        p[k][j] = __uint_as_float((__float_as_uint(p[k][j]) + (low & 0xFFFFu)) & 0xFFFF0000u);
+                    }
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const long long i = base + k * 128 + lane * 4;
+            if (whole) {
+                store4(pp + i, p[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (i + j < n) pp[i + j] = from_float<P>(p[k][j]);
+            }
+        }
+        if (!kF8) continue;
+        most_m = warp_most(most_m), most_r = warp_most(most_r);
+        const bool zm = most_m < 0x1p-100f, zr = most_r < 0x1p-100f;   // false for NaN
+        const float im = zm ? 0.0f : 448.0f / most_m, ir = zr ? 0.0f : 448.0f / most_r;
+        if (lane == 0)
+            *reinterpret_cast<float2*>(t.scales + base / 256 * 2) =
+                make_float2(zm ? 0.0f : most_m / 448.0f, zr ? 0.0f : most_r / 448.0f);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            cm[k] = cv[k] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                cm[k] |= encode(m[k][j] * im, stochastic, bits[k][j] & 0xFFFFu) << j * 8;
+                unsigned c = encode(v[k][j] * ir, stochastic, bits[k][j] >> 16);
+                if (!zr && v[k][j] > 0.0f) c = max(c, 1u);   // a moment above zero never divides by eps alone
+                cv[k] |= c << j * 8;
+            }
+            const long long i = base + k * 128 + lane * 4;
+            if (whole) {
+                __stcs(reinterpret_cast<uint32_t*>((unsigned char*)t.m + i), cm[k]);
+                __stcs(reinterpret_cast<uint32_t*>((unsigned char*)t.v + i), cv[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (i + j < n) {
+                        ((unsigned char*)t.m)[i + j] = (unsigned char)(cm[k] >> j * 8);
+                        ((unsigned char*)t.v)[i + j] = (unsigned char)(cv[k] >> j * 8);
+                    }
+            }
+        }
     }
 }
 
-// Each block's chunks, then the blocks' sums by one block, in 64 bits.
+// ---- norm -------------------------------------------------------------------------------
+__device__ __forceinline__ double square(float x) { return (double)x * (double)x; }
+
+// A block's sum over its chunks, on its first thread.
 template <class G, int N>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ List<N> list, double* sums, int more) {
-    __shared__ double buf[kThreads / 32];
+__device__ __forceinline__ double sum_squares(const List<N>& list, double* buf) {
     double s = 0.0;
     const unsigned chunks = list.first[list.count];
-    for (unsigned c = blockIdx.x; c < chunks; c += kNormBlocks) {
+    for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
         const int k = find(list, c);
         const Tensor& t = list.t[k];
-        const long long base = (long long)(c - list.first[k]) * kChunk;
-        for (int u = 0; u < 8; u++) {
-            const long long i = base + u * kThreads + threadIdx.x;
-            if (i < t.n) {
-                const double g = (double)to_float(((const G*)t.g)[i]);
-                s += g * g;
+        const G* g = (const G*)t.g;
+        const long long begin = (long long)(c - list.first[k]) * list.turns * kTurn;
+        for (int turn = 0; turn < list.turns; turn++) {
+            const long long base = begin + turn * kTurn;
+            if (base >= t.n) break;
+            if (t.even && base + kTurn <= t.n) {
+                float x[2][4];
+#pragma unroll
+                for (int u = 0; u < 2; u++) load4(x[u], g + base + (u * kThreads + threadIdx.x) * 4);
+#pragma unroll
+                for (int u = 0; u < 2; u++) s += (square(x[u][0]) + square(x[u][1])) + (square(x[u][2]) + square(x[u][3]));
+            } else {
+                for (int u = 0; u < 8; u++) {
+                    const long long i = base + u * kThreads + threadIdx.x;
+                    if (i < t.n) s += square(to_float(g[i]));
+                }
             }
         }
     }
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = s;
     __syncthreads();
+    if (threadIdx.x == 0)
+        for (int i = 1; i < kThreads / 32; i++) s += buf[i];
+    return s;
+}
+
+__device__ __forceinline__ void write_norm(double s, float max_norm, float* out) {
+    const float norm = (float)sqrt(s);
+    out[0] = norm;
+    out[1] = fabsf(norm) < kInf ? fminf(1.0f, max_norm / (norm + 1e-6f)) : norm - norm;
+}
+
+template <class G, int N>
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __grid_constant__ List<N> list, double* sums, int more) {
+    __shared__ double buf[kThreads / 32];
+    const double s = sum_squares<G>(list, buf);
+    if (threadIdx.x == 0) sums[blockIdx.x] = more ? sums[blockIdx.x] + s : s;
+}
+
+__global__ void __launch_bounds__(kThreads) norm_end_kernel(const double* sums, float max_norm, float* out) {
+    __shared__ double buf[kThreads / 32];
+    double s = 0.0;
+    for (int i = threadIdx.x; i < kNormBlocks; i += kThreads) s += sums[i];
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+    if (threadIdx.x % 32 == 0) buf[threadIdx.x / 32] = s;
+    __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < kThreads / 32; i++) s += buf[i];
-        sums[blockIdx.x] = more ? sums[blockIdx.x] + s : s;
+        write_norm(s, max_norm, out);
     }
 }
 
-__global__ void __launch_bounds__(32) norm_end_kernel(const double* sums, float max_norm, float* out) {
-    double s = 0.0;
-    for (int i = threadIdx.x; i < kNormBlocks; i += 32) s += sums[i];
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-    if (threadIdx.x == 0) {
-        const float norm = (float)sqrt(s);
-        out[0] = norm;
-        out[1] = fabsf(norm) < kInf ? fminf(1.0f, max_norm / (norm + 1e-6f)) : norm - norm;
+// Few elements: one cluster, whose first block joins the sums.
+constexpr int kNormCluster = 8;
+constexpr long long kNormSmall = 1 << 18;   // elements
+
+template <class G>
+__global__ void __launch_bounds__(kThreads) norm_small_kernel(const __grid_constant__ List<kFew> list, float max_norm, float* out) {
+    __shared__ double buf[kThreads / 32], sum;
+    const double s = sum_squares<G>(list, buf);
+    if (threadIdx.x == 0) sum = s;
+    asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        double all = s;
+        for (int r = 1; r < kNormCluster; r++) {
+            unsigned at;
+            double x;
+            asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((unsigned)__cvta_generic_to_shared(&sum)), "r"(r));
+            asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(x) : "r"(at) : "memory");
+            all += x;
+        }
+        write_norm(all, max_norm, out);
     }
+    asm volatile("barrier.cluster.arrive;\nbarrier.cluster.wait;" ::: "memory");
 }
 
 int bytes_of(int type) { return type == B3X_F32 ? 4 : type == B3X_E4M3 || type == B3X_U8 ? 1 : 2; }
@@ -184,8 +373,10 @@ bool at(const void* p, int bytes) { return p && (uintptr_t)p % bytes == 0; }
 
 // Fills lists of at most N tensors and hands each to `go`; tensors without elements are left out.
 template <int N, class Fill, class Go>
-int each_list(int count, const long long* sizes, Fill fill, Go go) {
-    static thread_local List<N> list;
+int each_list(int count, const long long* sizes, int turns, Fill fill, Go go) {
+    List<N> list;
+    list.turns = turns;
+    const long long chunk = (long long)turns * kTurn;
     int k = 0;
     bool more = false;
     while (k < count) {
@@ -193,7 +384,7 @@ int each_list(int count, const long long* sizes, Fill fill, Go go) {
         list.first[0] = 0;
         for (; k < count && list.count < N; k++) {
             if (sizes[k] == 0) continue;
-            const long long chunks = (sizes[k] + kChunk - 1) / kChunk;
+            const long long chunks = (sizes[k] + chunk - 1) / chunk;
             if (list.first[list.count] + chunks > 0x7fffffff) break;
             list.t[list.count] = fill(k);
             list.first[list.count + 1] = list.first[list.count] + (unsigned)chunks;
@@ -207,6 +398,16 @@ int each_list(int count, const long long* sizes, Fill fill, Go go) {
     }
     return (int)cudaSuccess;
 }
+
+// Chunks of one turn while there are few, so that all SMs have some.
+int turns_for(int count, const long long* sizes) {
+    long long all = 0;
+    for (int k = 0; k < count; k++) all += sizes[k];
+    return all / kTurn >= 148 * 32 ? 4 : 1;
+}
+
+// Whether p is at a multiple of 4 elements of `bytes` (or absent).
+int even(const void* p, int bytes) { return (uintptr_t)p % (4 * bytes) == 0; }
 
 bool sizes_ok(int count, const long long* sizes) {
     if (count < 0 || (count > 0 && !sizes)) return false;
@@ -228,22 +429,43 @@ int b3x_train_grad_norm_gpu(int count, const void* const* grads, int grad_type, 
         if (sizes[k] > 0 && !at(grads[k], bytes_of(grad_type))) return (int)cudaErrorInvalidValue;
     double* sums = (double*)workspace;
     const cudaStream_t s = (cudaStream_t)stream;
-    bool any = false;
-    const int e = each_list<kList>(
-        count, sizes,
-        [&](int k) { return Tensor{nullptr, grads[k], nullptr, nullptr, nullptr, nullptr, sizes[k], 0.0f, 0}; },
-        [&](const List<kList>& list, bool more) {
-            any = true;
-            if (grad_type == B3X_F32) norm_kernel<float><<<kNormBlocks, kThreads, 0, s>>>(list, sums, more);
-            if (grad_type == B3X_BF16) norm_kernel<__nv_bfloat16><<<kNormBlocks, kThreads, 0, s>>>(list, sums, more);
-            if (grad_type == B3X_F16) norm_kernel<__half><<<kNormBlocks, kThreads, 0, s>>>(list, sums, more);
-        });
-    if (e) return e;
-    if (!any) {
+    const int bytes = bytes_of(grad_type);
+    int used = 0;
+    long long all = 0;
+    for (int k = 0; k < count; k++) used += sizes[k] > 0, all += sizes[k];
+    auto fill = [&](int k) {
+        return Tensor{nullptr, grads[k], nullptr, nullptr, nullptr, nullptr, sizes[k], 0.0f, 0, even(grads[k], bytes)};
+    };
+    if (used == 0) {
         const cudaError_t z = cudaMemsetAsync(sums, 0, kNormBlocks * sizeof(double), s);
         if (z != cudaSuccess) return (int)z;
+    } else if (used <= kFew && all <= kNormSmall) {
+        cudaError_t e = cudaSuccess;
+        const int rc = each_list<kFew>(count, sizes, 1, fill, [&](const List<kFew>& list, bool) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(kNormCluster);
+            cfg.blockDim = dim3(kThreads);
+            cfg.stream = s;
+            cudaLaunchAttribute attribute[1];
+            attribute[0].id = cudaLaunchAttributeClusterDimension;
+            attribute[0].val.clusterDim.x = kNormCluster;
+            attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+            cfg.attrs = attribute;
+            cfg.numAttrs = 1;
+            const float limit = (float)max_norm;
+            if (grad_type == B3X_F32) e = cudaLaunchKernelEx(&cfg, norm_small_kernel<float>, list, limit, out);
+            if (grad_type == B3X_BF16) e = cudaLaunchKernelEx(&cfg, norm_small_kernel<__nv_bfloat16>, list, limit, out);
+            if (grad_type == B3X_F16) e = cudaLaunchKernelEx(&cfg, norm_small_kernel<__half>, list, limit, out);
+        });
+        return rc ? rc : (int)e;
     }
-    norm_end_kernel<<<1, 32, 0, s>>>(sums, (float)max_norm, out);
+    const int e = each_list<kMany>(count, sizes, turns_for(count, sizes), fill, [&](const List<kMany>& list, bool more) {
+        if (grad_type == B3X_F32) norm_kernel<float><<<kNormBlocks, kThreads, 0, s>>>(list, sums, more);
+        if (grad_type == B3X_BF16) norm_kernel<__nv_bfloat16><<<kNormBlocks, kThreads, 0, s>>>(list, sums, more);
+        if (grad_type == B3X_F16) norm_kernel<__half><<<kNormBlocks, kThreads, 0, s>>>(list, sums, more);
+    });
+    if (e) return e;
+    norm_end_kernel<<<1, kThreads, 0, s>>>(sums, (float)max_norm, out);
     return (int)cudaGetLastError();
 }
 
@@ -277,7 +499,10 @@ int b3x_train_adamw_gpu(int count, void* const* params, int param_type, const vo
         const double wd = decays ? (double)decays[k] : weight_decay;
         const unsigned key = mix(seed + (unsigned)k * 0x9E3779B1u + (unsigned)(unsigned long long)step * 0x6A09E667u);
         return Tensor{params[k], grads[k], exp_avg[k], exp_avg_sq[k], f8 ? scales[k] : nullptr,
-                      copies ? (__nv_bfloat16*)copies[k] : nullptr, sizes[k], (float)(1.0 - lr * wd), key};
+                      copies ? (__nv_bfloat16*)copies[k] : nullptr, sizes[k], (float)(1.0 - lr * wd), key,
+                      even(params[k], bytes_of(param_type)) && even(grads[k], bytes_of(grad_type)) &&
+                          even(exp_avg[k], bytes_of(state_type)) && even(exp_avg_sq[k], bytes_of(state_type)) &&
+                          even(copies ? copies[k] : nullptr, 2)};
     };
     auto go = [&](const auto& list, bool) {
         const unsigned grid = list.first[list.count];
@@ -295,5 +520,8 @@ int b3x_train_adamw_gpu(int count, void* const* params, int param_type, const vo
         }
 #undef B3T_GO
     };
-    return each_list<kList>(count, sizes, fill, go);
+    int used = 0;
+    for (int k = 0; k < count; k++) used += sizes[k] > 0;
+    const int turns = turns_for(count, sizes);
+    return used <= kFew ? each_list<kFew>(count, sizes, turns, fill, go) : each_list<kMany>(count, sizes, turns, fill, go);
 }
