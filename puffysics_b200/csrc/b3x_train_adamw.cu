@@ -89,14 +89,33 @@ __device__ __forceinline__ float2 decode2(unsigned codes) {
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// The e4m3 code of y.  Scaled by 2^-120 the format's exponents are float's,
-// subnormals included, so the code is the upper bits of the word; what is added
-// to the 20 bits below it rounds: random bits up or down in proportion, a half
-// to nearest.
-__device__ __forceinline__ unsigned encode(float y, bool stochastic, unsigned bits16) {
-    unsigned w = __float_as_uint(fabsf(y) * 0x1p-120f);
-    w += stochastic ? (bits16 << 4 | 8u) : 0x7FFFFu + ((w >> 20) & 1u);
-    return min(w >> 20, 0x7Eu) | (y < 0.0f ? 0x80u : 0u);
+// The e4m3 code of |y| in the upper byte.  Scaled by 2^-120 the format's
+// exponents are float's, subnormals included, so the code is the word from bit
+// 20 on; what is added to the 20 bits below it rounds: random bits up or down in
+// proportion (16 of them, and a half of the last), a half to nearest.
+template <bool kRandom>
+__device__ __forceinline__ uint32_t encode(float y, uint32_t bits16_at4, uint32_t least) {
+    uint32_t w = __float_as_uint(fabsf(y) * 0x1p-120f);
+    w += kRandom ? (bits16_at4 & 0xFFFF0u) | 8u : 0x7FFFFu + ((w >> 20) & 1u);
+    return max(min(w, 0x7EFFFFFu), least) << 4;
+}
+
+// The upper bytes of four words.
+__device__ __forceinline__ uint32_t upper_bytes(const uint32_t (&w)[4]) {
+    return __byte_perm(__byte_perm(w[0], w[1], 0x0073), __byte_perm(w[2], w[3], 0x0073), 0x5410);
+}
+
+// A sum of products that rounds by itself: a two-wide addition would be fused with one of them.
+__device__ __forceinline__ uint64_t sum2(uint64_t a, uint64_t b) {
+    const float2 x = unpack2(a), y = unpack2(b);
+    return pack2(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y));
+}
+
+// The largest of three numbers' magnitudes, NaN above all.
+__device__ __forceinline__ float most3(float a, float b, float c) {
+    float y;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
 }
 
 __device__ __forceinline__ float reciprocal(float x) {   // 1 ulp
@@ -114,9 +133,8 @@ __device__ __forceinline__ float warp_most(float x) {
 // so that every load and store is a whole line however wide its type.  The
 // moments' operations round one by one: their codes are those of the plain
 // formula, bit for bit.
-template <class P, class G, bool kF8, int N>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ List<N> list, const Hyper h,
-                                                         const int stochastic) {
+template <class P, class G, bool kF8, bool kRandom, int N>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ List<N> list, const Hyper h) {
     const float gs = h.grad_scale ? *h.grad_scale : 1.0f;
     if (!(fabsf(gs) < kInf)) return;
     const int which = find(list, blockIdx.x);
@@ -169,31 +187,42 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
                 }
             }
         }
-        float most_m = 0.0f, most_r = 0.0f;
+        float most_m = 0.0f, most_r = 0.0f, most_p = 0.0f;
+        const uint64_t gs2 = pack2(gs, gs), sm2 = pack2(sm, sm), sr2 = pack2(sr, sr), b1 = pack2(h.b1, h.b1),
+                       c1 = pack2(h.c1, h.c1), b2 = pack2(h.b2, h.b2), c2 = pack2(h.c2, h.c2), root = pack2(h.root, h.root),
+                       eps = pack2(h.eps, h.eps), keep = pack2(t.keep, t.keep), rate = pack2(-h.rate, -h.rate);
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            if (kF8) {
+        for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int j = 0; j < 4; j += 2) {
-                    const float2 a = decode2(cm[k] >> j * 8), b = decode2(cv[k] >> j * 8);
-                    m[k][j] = a.x * sm, m[k][j + 1] = a.y * sm;
-                    const float r0 = b.x * sr, r1 = b.y * sr;
-                    v[k][j] = r0 * r0, v[k][j + 1] = r1 * r1;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float x = g[k][j] * gs;
-                m[k][j] = m[k][j] * h.b1 + x * h.c1;
-                v[k][j] = v[k][j] * h.b2 + (x * x) * h.c2;
-                const float r = sqrtf(v[k][j]);
-                p[k][j] = p[k][j] * t.keep - (m[k][j] * reciprocal(r * h.root + h.eps)) * h.rate;
+            for (int j = 0; j < 4; j += 2) {
+                uint64_t m2, v2;
                 if (kF8) {
-                    most_m = max_nan(most_m, fabsf(m[k][j])), most_r = max_nan(most_r, r);
-                    v[k][j] = r;
+                    const float2 a = decode2(cm[k] >> j * 8), b = decode2(cv[k] >> j * 8);
+                    m2 = mul2(pack2(a.x, a.y), sm2);
+                    const uint64_t r = mul2(pack2(b.x, b.y), sr2);
+                    v2 = mul2(r, r);
+                } else {
+                    m2 = pack2(m[k][j], m[k][j + 1]);
+                    v2 = pack2(v[k][j], v[k][j + 1]);
                 }
+                const uint64_t x = mul2(pack2(g[k][j], g[k][j + 1]), gs2);
+                m2 = sum2(mul2(m2, b1), mul2(x, c1));
+                v2 = sum2(mul2(v2, b2), mul2(mul2(x, x), c2));
+                const float2 vv = unpack2(v2);
+                const float2 r = make_float2(sqrtf(vv.x), sqrtf(vv.y));
+                const float2 d = unpack2(add2(mul2(pack2(r.x, r.y), root), eps));
+                const uint64_t step = mul2(mul2(m2, pack2(reciprocal(d.x), reciprocal(d.y))), rate);
+                const float2 np = unpack2(add2(mul2(pack2(p[k][j], p[k][j + 1]), keep), step)), nm = unpack2(m2);
+                p[k][j] = np.x, p[k][j + 1] = np.y;
+                m[k][j] = nm.x, m[k][j + 1] = nm.y;
+                if (kF8) {
+                    most_m = most3(most_m, nm.x, nm.y), most_r = most3(most_r, r.x, r.y);
+                    v[k][j] = r.x, v[k][j + 1] = r.y;
+                } else {
+                    v[k][j] = vv.x, v[k][j + 1] = vv.y;
+                }
+                if (kRandom && sizeof(P) == 2) most_p = most3(most_p, np.x, np.y);
             }
-        }
         if (!kF8) {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
@@ -222,28 +251,52 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
             }
         }
         uint32_t bits[2][4];
-        if (stochastic && (kF8 || sizeof(P) == 2)) {
+        if (kRandom) {
+            const uint32_t at = (uint32_t)(base + lane * 4) * 0x9E3779B1u + (uint32_t)(base >> 32) * 0x6A09E667u + t.key;
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const long long i = base + k * 128 + lane * 4 + j;
-                    bits[k][j] = mix((unsigned)i * 0x9E3779B1u + (unsigned)(i >> 32) * 0x6A09E667u + t.key);
-                    if (sizeof(P) == 2 && fabsf(p[k][j]) < kInf) {
-                        const unsigned low = mix(bits[k][j] + 0x9E3779B1u);
-                        p[k][j] = __uint_as_float((__float_as_uint(p[k][j]) + (low & 0xFFFFu)) & 0xFFFF0000u);
-                    }
-                }
+                for (int j = 0; j < 4; j++) bits[k][j] = mix(at + (k * 128 + j) * 0x9E3779B1u);
         }
+        if (kRandom && sizeof(P) == 2) {
+            uint32_t low[2][4];
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const long long i = base + k * 128 + lane * 4;
-            if (whole) {
-                store4(pp + i, p[k]);
-            } else {
+            for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (i + j < n) pp[i + j] = from_float<P>(p[k][j]);
+                for (int j = 0; j < 4; j++) low[k][j] = mix(bits[k][j] + 0x9E3779B1u) & 0xFFFFu;
+            if (most_p != most_p) {   // NaN stays what it is
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (p[k][j] != p[k][j]) low[k][j] = 0;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const long long i = base + k * 128 + lane * 4;
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) w[j] = __float_as_uint(p[k][j]) + low[k][j];
+                const uint2 q = make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+                if (whole) {
+                    __stcs(reinterpret_cast<uint2*>(pp + i), q);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (i + j < n) reinterpret_cast<uint16_t*>(pp)[i + j] = (uint16_t)(w[j] >> 16);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const long long i = base + k * 128 + lane * 4;
+                if (whole) {
+                    store4(pp + i, p[k]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (i + j < n) pp[i + j] = from_float<P>(p[k][j]);
+                }
             }
         }
         if (!kF8) continue;
@@ -253,16 +306,18 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         if (lane == 0)
             *reinterpret_cast<float2*>(t.scales + base / 256 * 2) =
                 make_float2(zm ? 0.0f : most_m / 448.0f, zr ? 0.0f : most_r / 448.0f);
+        const uint32_t least = zr ? 0u : 1u << 20;   // a moment above zero never divides by eps alone
 #pragma unroll
         for (int k = 0; k < 2; k++) {
-            cm[k] = cv[k] = 0;
+            uint32_t wm[4], wv[4], sign[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                cm[k] |= encode(m[k][j] * im, stochastic, bits[k][j] & 0xFFFFu) << j * 8;
-                unsigned c = encode(v[k][j] * ir, stochastic, bits[k][j] >> 16);
-                if (!zr && v[k][j] > 0.0f) c = max(c, 1u);   // a moment above zero never divides by eps alone
-                cv[k] |= c << j * 8;
+                wm[j] = encode<kRandom>(m[k][j] * im, bits[k][j] << 4, 0u);
+                wv[j] = encode<kRandom>(v[k][j] * ir, bits[k][j] >> 12, min(__float_as_uint(v[k][j]), least));
+                sign[j] = __float_as_uint(m[k][j]);
             }
+            cm[k] = upper_bytes(wm) | (upper_bytes(sign) & 0x80808080u);
+            cv[k] = upper_bytes(wv);
             const long long i = base + k * 128 + lane * 4;
             if (whole) {
                 __stcs(reinterpret_cast<uint32_t*>((unsigned char*)t.m + i), cm[k]);
@@ -506,9 +561,11 @@ int b3x_train_adamw_gpu(int count, void* const* params, int param_type, const vo
     };
     auto go = [&](const auto& list, bool) {
         const unsigned grid = list.first[list.count];
-#define B3T_GO(P, G) \
-        (f8 ? adamw_kernel<P, G, true><<<grid, kThreads, 0, s>>>(list, h, stochastic) \
-            : adamw_kernel<P, G, false><<<grid, kThreads, 0, s>>>(list, h, stochastic))
+#define B3T_GO(P, G)                                                                                        \
+        (f8 ? stochastic ? adamw_kernel<P, G, true, true><<<grid, kThreads, 0, s>>>(list, h)                \
+                         : adamw_kernel<P, G, true, false><<<grid, kThreads, 0, s>>>(list, h)               \
+            : stochastic && sizeof(P) == 2 ? adamw_kernel<P, G, false, sizeof(P) == 2><<<grid, kThreads, 0, s>>>(list, h) \
+                         : adamw_kernel<P, G, false, false><<<grid, kThreads, 0, s>>>(list, h))
         if (param_type == B3X_F32) {
             if (grad_type == B3X_F32) B3T_GO(float, float);
             if (grad_type == B3X_BF16) B3T_GO(float, __nv_bfloat16);

@@ -322,28 +322,6 @@ template <> __device__ __forceinline__ float most<__half>(const uint4& q) {
     return max_nan(__low2float(a), __high2float(a));
 }
 
-// Two floats in one register pair, for the two-wide 32-bit arithmetic of sm_100.
-__device__ __forceinline__ uint64_t pack2(float x, float y) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-    return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t a) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-
 // U vectors' part of s and t.  What is -infinity is known only by the NaN it
 // leaves in t (0 times -infinity): then, and always with a mask, once more with
 // the exponents stopped, which costs an instruction a logit.
