@@ -89,15 +89,16 @@ __device__ __forceinline__ float2 decode2(unsigned codes) {
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// The e4m3 code of |y| in the upper byte.  Scaled by 2^-120 the format's
+// The e4m3 code of |y| <= 448 in the upper byte.  Scaled by 2^-120 the format's
 // exponents are float's, subnormals included, so the code is the word from bit
 // 20 on; what is added to the 20 bits below it rounds: random bits up or down in
-// proportion (16 of them, and a half of the last), a half to nearest.
+// proportion (16 of them, and a half of the last), a half to nearest.  448 and
+// its next neighbours, which a product may round to, never carry beyond the
+// largest code.
 template <bool kRandom>
-__device__ __forceinline__ uint32_t encode(float y, uint32_t bits16_at4, uint32_t least) {
-    uint32_t w = __float_as_uint(fabsf(y) * 0x1p-120f);
-    w += kRandom ? (bits16_at4 & 0xFFFF0u) | 8u : 0x7FFFFu + ((w >> 20) & 1u);
-    return max(min(w, 0x7EFFFFFu), least) << 4;
+__device__ __forceinline__ uint32_t encode(float y, uint32_t bits16_at4) {
+    const uint32_t w = __float_as_uint(fabsf(y) * 0x1p-120f);
+    return (w + (kRandom ? (bits16_at4 & 0xFFFF0u) | 8u : 0x7FFFFu + ((w >> 20) & 1u))) << 4;
 }
 
 // The upper bytes of four words.
@@ -134,7 +135,7 @@ __device__ __forceinline__ float warp_most(float x) {
 // moments' operations round one by one: their codes are those of the plain
 // formula, bit for bit.
 template <class P, class G, bool kF8, bool kRandom, int N>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ List<N> list, const Hyper h) {
+__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ List<N> list, const Hyper h) {
     const float gs = h.grad_scale ? *h.grad_scale : 1.0f;
     if (!(fabsf(gs) < kInf)) return;
     const int which = find(list, blockIdx.x);
@@ -306,18 +307,23 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
         if (lane == 0)
             *reinterpret_cast<float2*>(t.scales + base / 256 * 2) =
                 make_float2(zm ? 0.0f : most_m / 448.0f, zr ? 0.0f : most_r / 448.0f);
-        const uint32_t least = zr ? 0u : 1u << 20;   // a moment above zero never divides by eps alone
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             uint32_t wm[4], wv[4], sign[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                wm[j] = encode<kRandom>(m[k][j] * im, bits[k][j] << 4, 0u);
-                wv[j] = encode<kRandom>(v[k][j] * ir, bits[k][j] >> 12, min(__float_as_uint(v[k][j]), least));
+                wm[j] = encode<kRandom>(m[k][j] * im, bits[k][j] << 4);
+                wv[j] = encode<kRandom>(v[k][j] * ir, bits[k][j] >> 12);
                 sign[j] = __float_as_uint(m[k][j]);
             }
             cm[k] = upper_bytes(wm) | (upper_bytes(sign) & 0x80808080u);
             cv[k] = upper_bytes(wv);
+            // a moment above zero never becomes zero: it would divide by eps alone
+            if (((cv[k] + 0x7F7F7F7Fu) & 0x80808080u) != 0x80808080u && !zr) {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (v[k][j] > 0.0f && !(cv[k] >> j * 8 & 0xFFu)) cv[k] |= 1u << j * 8;
+            }
             const long long i = base + k * 128 + lane * 4;
             if (whole) {
                 __stcs(reinterpret_cast<uint32_t*>((unsigned char*)t.m + i), cm[k]);
