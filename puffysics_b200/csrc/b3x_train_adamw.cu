@@ -125,6 +125,22 @@ __device__ __forceinline__ float reciprocal(float x) {   // 1 ulp
     return y;
 }
 
+// Square roots of two numbers in [2^-96, 2^100], rounded as sqrtf rounds them:
+// Newton's step from s = v y, y an approximate 1 / sqrt(v), with the residual
+// v - s^2 formed by a fused operation (Markstein 1990).  What is left of the
+// error before the last rounding, about 2^-45, decides no rounding of a 24-bit
+// number (tried for all significands of two octaves).  sqrtf's own cases for
+// other numbers cost a branch a number.
+__device__ __forceinline__ uint64_t sqrt2(uint64_t v) {
+    const float2 x = unpack2(v);
+    float2 y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(x.x));
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(x.y));
+    const uint64_t y2 = pack2(y.x, y.y), s = mul2(v, y2), minus = mul2(s, pack2(-1.0f, -1.0f));
+    const uint64_t half = mul2(y2, pack2(0.5f, 0.5f));
+    return fma2(fma2(minus, s, v), half, s);
+}
+
 // The largest of a warp's numbers that are not negative; NaN is the largest.
 __device__ __forceinline__ float warp_most(float x) {
     return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(x) & 0x7FFFFFFFu));
@@ -210,10 +226,12 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
                 m2 = sum2(mul2(m2, b1), mul2(x, c1));
                 v2 = sum2(mul2(v2, b2), mul2(mul2(x, x), c2));
                 const float2 vv = unpack2(v2);
-                const float2 r = make_float2(sqrtf(vv.x), sqrtf(vv.y));
-                const float2 d = unpack2(add2(mul2(pack2(r.x, r.y), root), eps));
+                float2 r;
+                if (fminf(vv.x, vv.y) >= 0x1p-96f && fmaxf(vv.x, vv.y) <= 0x1p100f) r = unpack2(sqrt2(v2));
+                else r = make_float2(sqrtf(vv.x), sqrtf(vv.y));
+                const float2 d = unpack2(fma2(pack2(r.x, r.y), root, eps));
                 const uint64_t step = mul2(mul2(m2, pack2(reciprocal(d.x), reciprocal(d.y))), rate);
-                const float2 np = unpack2(add2(mul2(pack2(p[k][j], p[k][j + 1]), keep), step)), nm = unpack2(m2);
+                const float2 np = unpack2(fma2(pack2(p[k][j], p[k][j + 1]), keep, step)), nm = unpack2(m2);
                 p[k][j] = np.x, p[k][j + 1] = np.y;
                 m[k][j] = nm.x, m[k][j + 1] = nm.y;
                 if (kF8) {
@@ -302,11 +320,11 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
         }
         if (!kF8) continue;
         most_m = warp_most(most_m), most_r = warp_most(most_r);
-        const bool zm = most_m < 0x1p-100f, zr = most_r < 0x1p-100f;   // false for NaN
-        const float im = zm ? 0.0f : 448.0f / most_m, ir = zr ? 0.0f : 448.0f / most_r;
-        if (lane == 0)
-            *reinterpret_cast<float2*>(t.scales + base / 256 * 2) =
-                make_float2(zm ? 0.0f : most_m / 448.0f, zr ? 0.0f : most_r / 448.0f);
+        // a division for each quarter of the lanes: the scales, and what makes codes of the moments
+        const float most = lane < 16 ? most_m : most_r;
+        const float part = most < 0x1p-100f ? 0.0f : lane & 8 ? 448.0f / most : most / 448.0f;
+        if ((lane & 15) == 0) t.scales[base / 256 * 2 + lane / 16] = part;
+        const float im = __shfl_sync(~0u, part, 8), ir = __shfl_sync(~0u, part, 24);
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             uint32_t wm[4], wv[4], sign[4];
@@ -319,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
             cm[k] = upper_bytes(wm) | (upper_bytes(sign) & 0x80808080u);
             cv[k] = upper_bytes(wv);
             // a moment above zero never becomes zero: it would divide by eps alone
-            if (((cv[k] + 0x7F7F7F7Fu) & 0x80808080u) != 0x80808080u && !zr) {
+            if (((cv[k] + 0x7F7F7F7Fu) & 0x80808080u) != 0x80808080u && ir != 0.0f) {
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (v[k][j] > 0.0f && !(cv[k] >> j * 8 & 0xFFu)) cv[k] |= 1u << j * 8;
