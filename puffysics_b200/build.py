@@ -39,9 +39,10 @@ THREAD_DEPS = THREAD_HEADERS + [os.path.join(ROOT, "include", "puffysics_b200.h"
                                 os.path.join(PKG, "csrc", "b3x_math.cuh"), os.path.join(PKG, "csrc", "b3x_narrow.cuh"),
                                 os.path.join(PKG, "scenes", "b3_scenes.h")]
 # the training operators (libb3train.so)
-TRAIN_SRC = [os.path.join(PKG, "csrc", "b3x_train_%s.cu" % n) for n in ("logprob", "advantage", "adamw")]
+TRAIN_SRC = [os.path.join(PKG, "csrc", "b3x_train_%s.cu" % n) for n in ("logprob", "logprob_grad", "advantage", "adamw")]
 TRAIN_LIB = os.path.join(LIB_DIR, "libb3train.so")
-TRAIN_HEADERS = [os.path.join(ROOT, "include", "b3x_train.h"), os.path.join(PKG, "csrc", "b3x_train_common.cuh")]
+TRAIN_HEADERS = [os.path.join(ROOT, "include", "b3x_train.h"), os.path.join(PKG, "csrc", "b3x_train_common.cuh"),
+                 os.path.join(PKG, "csrc", "b3x_train_rows.cuh")]
 # capacity configurations the host scene builders are compiled for:
 # name -> (bodies, shapes, contacts, joints)
 SCENE_CONFIGS = {"hover": (2, 2, 4, 1), "stack": (9, 9, 32, 1), "chain": (12, 12, 32, 10),

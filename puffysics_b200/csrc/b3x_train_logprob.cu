@@ -1,33 +1,12 @@
 // b3x_train_logprob.cu -- log probabilities of actions, entropies and most
-// likely alternatives of rows of logits, and their gradient (b3x_train.h).
-#include <cmath>
+// likely alternatives of rows of logits (b3x_train.h).
+#include <type_traits>
 
-#include "b3x_train_common.cuh"
+#include "b3x_train_rows.cuh"
 
 using namespace b3t;
 
 namespace {
-
-struct Rows {
-    const void* logits;
-    long long rows, row_stride;
-    const unsigned char* mask;
-    long long mask_stride;
-    const void* actions;
-    int action_bytes, width;
-    float scale;
-};
-
-__device__ __forceinline__ long long action_of(const Rows& a, long long row) {
-    if (!a.actions) return -1;
-    return a.action_bytes == 8 ? ((const long long*)a.actions)[row] : (long long)((const int*)a.actions)[row];
-}
-
-template <class T>
-__device__ __forceinline__ float logit(const Rows& a, long long row, int j) {
-    if (a.mask && !a.mask[row * a.mask_stride + j]) return -kInf;
-    return to_float(((const T*)a.logits)[row * a.row_stride + j]);
-}
 
 struct Out {
     float *logp, *entropy, *stats;
@@ -130,196 +109,49 @@ __device__ __forceinline__ void write_row(const Rows& a, const Out& o, long long
     }
 }
 
-// ---- short rows -------------------------------------------------------------------------
-// Up to 8 logits a lane, L lanes a row, all in registers: bound by latency and
-// by the words a row has besides its logits.
-constexpr int kShort = 8;
-constexpr int kShortThreads = 256;
+__device__ __forceinline__ void write_top(const Out& o, long long row, int k, uint64_t e, const Row& r, float scale) {
+    o.top_ids[row * o.top + k] = e ? index_of(e) : -1;
+    o.top_logp[row * o.top + k] = e ? r.logp(of_key((uint32_t)(e >> 32)), scale) : -kInf;
+}
 
-template <class T, int L>
+// ---- rows of a thread ---------------------------------------------------------------------
+// Up to 8 logits, one thread a row, all in registers: bound by the launch and by
+// the words that a row has besides its logits.
+constexpr int kShort = 8;
+constexpr int kShortThreads = 128;
+
+template <class T>
 __global__ void __launch_bounds__(kShortThreads) short_kernel(Rows a, Out o) {
-    const long long row = ((long long)blockIdx.x * kShortThreads + threadIdx.x) / L;
-    const int lane = threadIdx.x % L;
-    const bool on = row < a.rows;
+    const long long row = (long long)blockIdx.x * kShortThreads + threadIdx.x;
+    if (row >= a.rows) return;
     float z[kShort];
-    float m = -kInf;
+    Part p{-kInf, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kShort; i++) {
-        const int j = lane + i * L;
-        z[i] = on && j < a.width ? logit<T>(a, row, j) : -kInf;
-        m = max_nan(m, z[i]);
+        z[i] = i < a.width ? logit<T>(a, row, i) : -kInf;
+        p.m = max_nan(p.m, z[i]);
     }
-    for (int k = L / 2; k; k >>= 1) m = max_nan(m, __shfl_xor_sync(~0u, m, k));
     const float c = a.scale * kLog2e;
-    Part p{m, 0.0f, 0.0f, 0.0f};   // the maximum is known before the sums: x = c (z - m)
 #pragma unroll
-    for (int i = 0; i < kShort; i++) {
-        const float x = fmaxf((z[i] - m) * c, -1e4f), e = exp2_fast(x);
+    for (int i = 0; i < kShort; i++) {   // the maximum is known before the sums: x = c (z - m)
+        const float x = fmaxf((z[i] - p.m) * c, -1e4f), e = exp2_fast(x);
         p.s += e;
         p.t = __fmaf_rn(e, x, p.t);
     }
-    for (int k = L / 2; k; k >>= 1) p.s += __shfl_xor_sync(~0u, p.s, k), p.t += __shfl_xor_sync(~0u, p.t, k);
     const Row r = Row::about_maximum(p);
-    if (on && lane == 0) write_row<T>(a, o, row, r);
+    write_row<T>(a, o, row, r);
     uint64_t last = ~0ull;
     for (int k = 0; k < o.top; k++) {
         uint64_t best = 0;
 #pragma unroll
         for (int i = 0; i < kShort; i++) {
             const uint32_t key = key_of(z[i]);
-            const uint64_t e = entry_of(key, lane + i * L);
+            const uint64_t e = entry_of(key, i);
             if (key > kNothing && key <= kMost && e < last && e > best) best = e;
         }
-        for (int q = L / 2; q; q >>= 1) {
-            const uint64_t other = __shfl_xor_sync(~0u, best, q);
-            best = other > best ? other : best;
-        }
         last = best;
-        if (on && lane == k % L) {
-            const bool none = best == 0;
-            o.top_ids[row * o.top + k] = none ? -1 : index_of(best);
-            o.top_logp[row * o.top + k] = none ? -kInf : r.logp(of_key((uint32_t)(best >> 32)), a.scale);
-        }
+        write_top(o, row, k, best, r, a.scale);
     }
-}
-
-// ---- long rows --------------------------------------------------------------------------
-// 16 bytes of consecutive logits.  A row is cut on the 16-byte boundaries of
-// memory, wherever it starts: vector v holds the elements from v N - head on.
-template <class T> struct Vec { static constexpr int n = 16 / sizeof(T); };
-
-__device__ __forceinline__ uint4 load16(const void* p) {
-    uint4 q;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
-    return q;
-}
-
-template <class T> __device__ __forceinline__ uint32_t minus_infinity();
-template <> __device__ __forceinline__ uint32_t minus_infinity<float>() { return 0xFF800000u; }
-template <> __device__ __forceinline__ uint32_t minus_infinity<__nv_bfloat16>() { return 0xFF80FF80u; }
-template <> __device__ __forceinline__ uint32_t minus_infinity<__half>() { return 0xFC00FC00u; }
-
-// 0xFF in each byte that is not 0, as the sign bits of a word's bytes.
-__device__ __forceinline__ uint32_t nonzero_bytes(uint32_t x) { return ((x & 0x7F7F7F7Fu) + 0x7F7F7F7Fu) | x; }
-
-template <class T, bool kMask>
-struct Source {
-    const T* row;
-    const unsigned char* mask;
-    int width, head;
-
-    __device__ __forceinline__ Source(const Rows& a, long long r) {
-        row = (const T*)a.logits + r * a.row_stride;
-        mask = kMask ? a.mask + r * a.mask_stride : nullptr;
-        width = a.width;
-        head = (int)((uintptr_t)row % 16 / sizeof(T));
-    }
-    __device__ __forceinline__ int vectors() const { return (head + width + Vec<T>::n - 1) / Vec<T>::n; }
-
-    // Vectors [2, last) and two words beside them are inside the row.
-    __device__ __forceinline__ int last() const { return (head + width) / Vec<T>::n - 1; }
-    // A vector among those.
-    __device__ __forceinline__ uint4 inner(int v) const {
-        const int j = v * Vec<T>::n - head;
-        uint4 q = load16(row + j);
-        if (kMask) keep(q, mask + j);
-        return q;
-    }
-
-    // Vector v, -infinity where it is outside the row or masked.
-    __device__ __forceinline__ uint4 load(int v) const {
-        constexpr int N = Vec<T>::n;
-        const int j = v * N - head;
-        if (j >= 0 && j + N <= width) {
-            uint4 q = load16(row + j);
-            if (kMask) apply(q, j);
-            return q;
-        }
-        uint32_t w[4] = {minus_infinity<T>(), minus_infinity<T>(), minus_infinity<T>(), minus_infinity<T>()};
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            if (j + i < 0 || j + i >= width || (kMask && !mask[j + i])) continue;
-            if (sizeof(T) == 4) w[i % 4] = reinterpret_cast<const uint32_t*>(row)[j + i];
-            else {
-                const uint32_t x = reinterpret_cast<const uint16_t*>(row)[j + i];
-                w[i / 2 % 4] = i % 2 ? (w[i / 2 % 4] & 0xFFFFu) | x << 16 : (w[i / 2 % 4] & 0xFFFF0000u) | x;
-            }
-        }
-        return make_uint4(w[0], w[1], w[2], w[3]);
-    }
-
-    // Mask bytes j on, where the words around them may lie outside the row's own.
-    __device__ __forceinline__ void apply(uint4& q, int j) const {
-        constexpr int N = Vec<T>::n;
-        const int off = (int)((uintptr_t)(mask + j) & 3);
-        if (j >= off && j - off + N + 4 <= width) return keep(q, mask + j);
-        uint32_t b[2] = {0, 0};
-#pragma unroll
-        for (int i = 0; i < N; i++) b[i / 4] |= (uint32_t)mask[j + i] << i % 4 * 8;
-        keep(q, b);
-    }
-
-    // The N mask bytes at p, from the whole words around them.
-    static __device__ __forceinline__ void keep(uint4& q, const unsigned char* p) {
-        constexpr int N = Vec<T>::n;
-        const int off = (int)((uintptr_t)p & 3);
-        const uint32_t* w = reinterpret_cast<const uint32_t*>(p - off);
-        const uint32_t w0 = __ldg(w), w1 = N == 8 || off ? __ldg(w + 1) : 0u, w2 = N == 8 && off ? __ldg(w + 2) : 0u;
-        uint32_t b[2] = {__funnelshift_r(w0, w1, off * 8), __funnelshift_r(w1, w2, off * 8)};
-        keep(q, b);
-    }
-
-    static __device__ __forceinline__ void keep(uint4& q, uint32_t (&b)[2]) {
-        uint32_t* w = &q.x;
-        b[0] = nonzero_bytes(b[0]);
-        if (Vec<T>::n == 4) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) w[i] = b[0] >> i * 8 & 0x80u ? w[i] : minus_infinity<T>();
-        } else {
-            b[1] = nonzero_bytes(b[1]);
-#pragma unroll
-            for (int i = 0; i < 4; i++) {   // a byte's sign bit becomes 16 bits of ones
-                uint32_t ones;
-                asm("prmt.b32 %0, %1, 0, %2;" : "=r"(ones) : "r"(b[i / 2]), "r"(i % 2 ? 0xBBAA : 0x9988));
-                w[i] = (w[i] & ones) | (minus_infinity<T>() & ~ones);
-            }
-        }
-    }
-};
-
-// The two logits of word i (one for float, the other -infinity).
-template <class T> __device__ __forceinline__ float2 pair(uint32_t w);
-template <> __device__ __forceinline__ float2 pair<__nv_bfloat16>(uint32_t w) {
-    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-template <> __device__ __forceinline__ float2 pair<__half>(uint32_t w) {
-    return __half22float2(*reinterpret_cast<__half2*>(&w));
-}
-
-// Element i of a vector.
-template <class T> __device__ __forceinline__ float element(const uint4& q, int i) {
-    const uint32_t* w = &q.x;
-    if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
-    else {
-        const float2 f = pair<T>(w[i / 2]);
-        return i % 2 ? f.y : f.x;
-    }
-}
-
-template <class T> __device__ __forceinline__ float most(const uint4& q);
-template <> __device__ __forceinline__ float most<float>(const uint4& q) {
-    return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)), max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
-}
-template <> __device__ __forceinline__ float most<__nv_bfloat16>(const uint4& q) {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&q);
-    const __nv_bfloat162 a = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-    return max_nan(__low2float(a), __high2float(a));
-}
-template <> __device__ __forceinline__ float most<__half>(const uint4& q) {
-    const __half2* h = reinterpret_cast<const __half2*>(&q);
-    const __half2 a = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
-    return max_nan(__low2float(a), __high2float(a));
 }
 
 // U vectors' part of s and t.  What is -infinity is known only by the NaN it
@@ -363,10 +195,6 @@ __device__ __forceinline__ float most_of(const uint4 (&q)[U]) {
     return m;
 }
 
-template <class T> __device__ __forceinline__ uint4 no_vector() {
-    return make_uint4(minus_infinity<T>(), minus_infinity<T>(), minus_infinity<T>(), minus_infinity<T>());
-}
-
 // The lanes' keys from the largest down.
 __device__ __forceinline__ uint32_t sort_lanes(uint32_t key) {
     const int lane = threadIdx.x % 32;
@@ -394,11 +222,6 @@ __device__ __forceinline__ uint32_t merge_lanes(uint32_t key, uint32_t mirrored)
     return key;
 }
 
-__device__ __forceinline__ void write_top(const Out& o, long long row, int k, uint64_t e, const Row& r, float scale) {
-    o.top_ids[row * o.top + k] = e ? index_of(e) : -1;
-    o.top_logp[row * o.top + k] = e ? r.logp(of_key((uint32_t)(e >> 32)), scale) : -kInf;
-}
-
 // The sums of a row of logits of 1e38, whose products with c are beyond the
 // floats: x = c (z - m).  `by`: threads that share the row.
 template <class T, bool kMask>
@@ -416,84 +239,190 @@ __device__ __noinline__ float2 far_sums(const Source<T, kMask>& src, float m, fl
     return make_float2(s, t);
 }
 
-// ---- rows of a warp -----------------------------------------------------------------------
-// Rows of up to 32 U vectors, one a warp, kept in registers.  The K-th largest of
-// the lanes' maxima is at most the K-th largest logit: what reaches it is ranked.
-constexpr int kRowWarps = 8;
-constexpr int kRowFound = 160;
+// ---- rows of some lanes -------------------------------------------------------------------
+// Rows of up to 4 L vectors, L lanes a row, in registers.  Or (kWalk, 32 lanes)
+// of more, which the warp walks over twice when alternatives are asked for, the
+// second time from L2.
+//
+// Alternatives: a threshold that K logits reach, then what reaches it is ranked.
+// With 32 lanes it is the K-th largest of the lanes' maxima, with fewer that of
+// the vectors'.
+constexpr int kRowThreads = 256;
+constexpr int kRowFound = 256;       // logits that are ranked at once, for a warp's rows together
 
-template <class T, bool kMask, bool kTop, int U>
-__global__ void __launch_bounds__(kRowWarps * 32) row_kernel(Rows a, Out o) {
-    constexpr int N = Vec<T>::n;
-    __shared__ uint64_t entries[kTop ? kRowWarps : 1][kTop ? kRowFound : 1];
-    __shared__ int found[kRowWarps];
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const long long row = (long long)blockIdx.x * kRowWarps + warp;
-    if (row >= a.rows) return;
-    const Source<T, kMask> src(a, row);
-    const int nv = src.vectors();
-    const float c = a.scale * kLog2e;
-    uint4 q[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) q[u] = u * 32 + lane < nv ? src.load(u * 32 + lane) : no_vector<T>();
-    const float mine = most_of<T, U>(q);
-    Part p = empty_part();
-    p.m = warp_max(mine);
-    p.r = reference(p.m, c);
-    add_vectors<T, U, kMask>(q, c, p);
-    for (int k = 16; k; k >>= 1) p.s += __shfl_xor_sync(~0u, p.s, k), p.t += __shfl_xor_sync(~0u, p.t, k);
-    const bool far = out_of_range(p);
-    if (far) {
-        const float2 st = far_sums(src, p.m, c, lane, 32);
-        p.s = st.x, p.t = st.y;
-    }
-    const Row r = far ? Row::about_maximum(p) : Row(p, c);
-    if (lane == 0) write_row<T>(a, o, row, r);
-    if (!kTop) return;
-    const uint32_t sorted = sort_lanes(key_of(mine));
-    const uint32_t threshold = max(__shfl_sync(~0u, sorted, o.top - 1), kNothing + 1);
-    if (lane == 0) found[warp] = 0;
-    __syncwarp();
+// A bit for each logit of U vectors that reaches z: bit 4 u + i for word i of
+// vector u, and from bit 16 on for the words' upper halves.
+template <class T, int U>
+__device__ __forceinline__ uint32_t reach(const uint4 (&q)[U], float z) {
+    uint32_t bits = 0;
 #pragma unroll
     for (int u = 0; u < U; u++) {
-        if (key_of(most<T>(q[u])) < threshold) continue;
+        const uint32_t* w = &q[u].x;
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            const uint32_t key = key_of(element<T>(q[u], n));
-            if (key < threshold) continue;
-            const int at = atomicAdd(&found[warp], 1);
-            if (at < kRowFound) entries[warp][at] = entry_of(key, (u * 32 + lane) * N - src.head + n);
+        for (int i = 0; i < 4; i++) {
+            const uint32_t one = 0x00010001u << (u * 4 + i);
+            if constexpr (sizeof(T) == 4) {
+                if (__uint_as_float(w[i]) >= z) bits |= one & 0xFFFFu;
+            } else if constexpr (sizeof(T) == 2 && Vec<T>::n == 8) {
+                uint32_t m;
+                if constexpr (std::is_same<T, __nv_bfloat16>::value) m = __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), __float2bfloat162_rn(z));
+                else m = __hge2_mask(*reinterpret_cast<const __half2*>(&w[i]), __float2half2_rn(z));
+                bits |= m & one;
+            }
+        }
+    }
+    return bits;
+}
+
+// The lowest value of type T: what -infinity does not reach.
+template <class T> __device__ __forceinline__ float lowest();
+template <> __device__ __forceinline__ float lowest<float>() { return -3.402823466e38f; }
+template <> __device__ __forceinline__ float lowest<__nv_bfloat16>() { return __uint_as_float(0xFF7F0000u); }
+template <> __device__ __forceinline__ float lowest<__half>() { return -65504.0f; }
+
+
+template <class T, bool kMask, bool kTop, int L, bool kWalk>
+__global__ void __launch_bounds__(kRowThreads, kTop ? 3 : 4) lanes_kernel(Rows a, Out o) {
+    constexpr int N = Vec<T>::n, U = 4, kRows = 32 / L, kCap = kRowFound / kRows;
+    __shared__ uint64_t entries[kTop ? kRowThreads / L : 1][kTop ? kCap : 1];
+    __shared__ __align__(16) uint32_t best[kTop && L < 32 ? kRowThreads / L : 1][kTop && L < 32 ? U * L : 1];
+    __shared__ int found[kTop ? kRowThreads / L : 1];
+    const int here = threadIdx.x / L, lane = threadIdx.x % L;
+    const long long row = (long long)blockIdx.x * (kRowThreads / L) + here;
+    const bool on = row < a.rows;
+    const Source<T, kMask> src(a, on ? row : 0);
+    const int nv = on ? src.vectors() : 0;
+    const float c = a.scale * kLog2e;
+    if (kTop && lane == 0) found[here] = 0;
+    uint4 q[U];
+    const auto load = [&](int base) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int v = base + u * L + lane;
+            q[u] = v < nv ? src.load(v) : no_vector<T>();
+        }
+    };
+    Part p = empty_part();
+    float mine = -kInf;
+    if (kWalk) {
+        for (int base = 0; base < nv; base += U * L) {
+            if (base >= 2 && base + U * L <= src.last()) {
+#pragma unroll
+                for (int u = 0; u < U; u++) q[u] = src.inner(base + u * L + lane);
+            } else {
+                load(base);
+            }
+            const float m = max_nan(p.m, most_of<T, U>(q));
+            p = moved(p, m, reference(m, c));
+            add_vectors<T, U, kMask>(q, c, p);
+        }
+        mine = p.m;
+        p = join_lanes(p);
+    } else {
+        load(0);
+        p.m = mine = most_of<T, U>(q);
+#pragma unroll
+        for (int k = L / 2; k; k /= 2) p.m = max_nan(p.m, __shfl_xor_sync(~0u, p.m, k));
+        p.r = reference(p.m, c);
+        add_vectors<T, U, kMask>(q, c, p);
+#pragma unroll
+        for (int k = L / 2; k; k /= 2) p.s += __shfl_xor_sync(~0u, p.s, k), p.t += __shfl_xor_sync(~0u, p.t, k);
+    }
+    const bool far = out_of_range(p);
+    if (__any_sync(~0u, far)) {   // logits of 1e38: x = c (z - m)
+        float s = 0.0f, t = 0.0f;
+        for (int v = lane; v < nv; v += L) {
+            const uint4 w = src.load(v);
+            for (int n = 0; n < N; n++) {
+                const float x = fmaxf((element<T>(w, n) - p.m) * c, -1e4f), e = exp2_fast(x);
+                s += e;
+                t = __fmaf_rn(e, x, t);
+            }
+        }
+        for (int k = L / 2; k; k /= 2) s += __shfl_xor_sync(~0u, s, k), t += __shfl_xor_sync(~0u, t, k);
+        if (far) p.s = s, p.t = t;
+    }
+    const Row r = far ? Row::about_maximum(p) : Row(p, c);
+    if (on && lane == 0) write_row<T>(a, o, row, r);
+    if (!kTop) return;
+
+    float z;
+    if (L == 32) {
+        z = of_key(__shfl_sync(~0u, sort_lanes(key_of(mine)), o.top - 1));
+    } else {
+        uint32_t key[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) best[here][u * L + lane] = key[u] = key_of(most<T>(q[u]));
+        __syncwarp();
+        int above[U] = {};
+        const uint4* all = reinterpret_cast<const uint4*>(best[here]);
+        for (int i = 0; i < U * L / 4; i++) {
+            const uint4 w = all[i];
+#pragma unroll
+            for (int u = 0; u < U; u++) above[u] += (w.x > key[u]) + (w.y > key[u]) + (w.z > key[u]) + (w.w > key[u]);
+        }
+        // the least of those that fewer than K are above
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (above[u] >= o.top) key[u] = ~0u;
+        uint32_t least = min(min(key[0], key[1]), min(key[2], key[3]));
+#pragma unroll
+        for (int k = L / 2; k; k /= 2) least = min(least, __shfl_xor_sync(~0u, least, k));
+        z = o.top <= U * L ? of_key(least) : -kInf;   // too few vectors: every logit
+    }
+    z = fmaxf(z, lowest<T>());
+    __syncwarp();
+    for (int base = 0; base < (kWalk ? nv : 1); base += U * L) {
+        if (kWalk) load(base);
+        uint32_t bits = reach<T, U>(q, z);
+        if (bits) {
+            int at = atomicAdd(&found[here], __popc(bits));
+            while (bits) {
+                const int b = __ffs(bits) - 1, w = b & 15;
+                bits &= bits - 1;
+                if (at < kCap) entries[here][at] = (base + (w >> 2) * L + lane) * N - src.head + (w & 3) * (N / 4) + (b >> 4);
+                at++;
+            }
         }
     }
     __syncwarp();
-    const int n = found[warp];
-    if (n <= kRowFound && p.m == p.m) {
-        for (int i = lane; i < n; i += 32) {
-            const uint64_t e = entries[warp][i];
+    const int n = found[here];
+    const bool ranked = n <= kCap && p.m == p.m;
+    if (ranked) {
+        for (int i = lane; i < n; i += L) {
+            const int j = (int)entries[here][i];
+            entries[here][i] = entry_of(key_of(to_float(src.row[j])), j);
+        }
+    }
+    __syncwarp();
+    if (ranked && on) {
+        for (int i = lane; i < n; i += L) {
+            const uint64_t e = entries[here][i];
             int rank = 0;
-            for (int j = 0; j < n; j++) rank += entries[warp][j] > e;
+            for (int j = 0; j < n; j++) rank += entries[here][j] > e;
             if (rank < o.top) write_top(o, row, rank, e, r, a.scale);
         }
-        if (lane >= n && lane < o.top) write_top(o, row, lane, 0, r, a.scale);
-        return;
+        for (int i = n + lane; i < o.top; i += L) write_top(o, row, i, 0, r, a.scale);
     }
+    if (__all_sync(~0u, ranked)) return;
     // many equal logits, or NaN: each time the best one after the last
     uint64_t last = ~0ull;
     for (int k = 0; k < o.top; k++) {
-        uint64_t best = 0;
-#pragma unroll
-        for (int u = 0; u < U; u++)
+        uint64_t top = 0;
+        for (int v = lane; v < nv; v += L) {
+            const uint4 x = src.load(v);
             for (int i = 0; i < N; i++) {
-                const uint32_t key = key_of(element<T>(q[u], i));
-                const uint64_t e = entry_of(key, (u * 32 + lane) * N - src.head + i);
-                if (key > kNothing && key <= kMost && e < last && e > best) best = e;
+                const uint32_t key = key_of(element<T>(x, i));
+                const uint64_t e = entry_of(key, v * N - src.head + i);
+                if (key > kNothing && key <= kMost && e < last && e > top) top = e;
             }
-        for (int d = 16; d; d >>= 1) {
-            const uint64_t other = __shfl_xor_sync(~0u, best, d);
-            best = other > best ? other : best;
         }
-        last = best;
-        if (lane == 0) write_top(o, row, k, best, r, a.scale);
+        for (int d = L / 2; d; d /= 2) {
+            const uint64_t other = __shfl_xor_sync(~0u, top, d);
+            top = other > top ? other : top;
+        }
+        last = top;
+        if (on && !ranked && lane == 0) write_top(o, row, k, top, r, a.scale);
     }
 }
 
@@ -771,25 +700,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, 
 }
 static_assert(kMaxCluster * B3X_TRAIN_MAX_TOP <= kFound, "the blocks' alternatives are ranked at once");
 
-template <class T, int L>
-int launch_short(const Rows& a, const Out& o, cudaStream_t s) {
-    const long long per = kShortThreads / L;
-    short_kernel<T, L><<<(unsigned)((a.rows + per - 1) / per), kShortThreads, 0, s>>>(a, o);
-    return (int)cudaGetLastError();
-}
-
 template <class T, bool kMask, bool kTop>
-int launch_long(const Rows& a, const Out& o, cudaStream_t s) {
-    // the most vectors that a row has
-    const bool even = (uintptr_t)a.logits % 16 == 0 && a.row_stride * (long long)sizeof(T) % 16 == 0;
-    const int nv = (int)(((long long)a.width + Vec<T>::n - 1) / Vec<T>::n) + (even ? 0 : 1);
-    if (nv <= 4 * 32) {
-        const unsigned grid = (unsigned)((a.rows + kRowWarps - 1) / kRowWarps);
-        if (nv <= 32) row_kernel<T, kMask, kTop, 1><<<grid, kRowWarps * 32, 0, s>>>(a, o);
-        else if (nv <= 64) row_kernel<T, kMask, kTop, 2><<<grid, kRowWarps * 32, 0, s>>>(a, o);
-        else row_kernel<T, kMask, kTop, 4><<<grid, kRowWarps * 32, 0, s>>>(a, o);
-        return (int)cudaGetLastError();
-    }
+int launch_long(const Rows& a, const Out& o, int nv, cudaStream_t s) {
     // a cluster a row while rows alone leave SMs idle and each block keeps 512 vectors
     int cluster = 1;
     while (cluster < kMaxCluster && a.rows * cluster * 2 <= 296 && nv / (cluster * 2) >= 512) cluster *= 2;
@@ -819,58 +731,40 @@ int launch_long(const Rows& a, const Out& o, cudaStream_t s) {
     return (int)cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, false>, a, o, cluster, shift);
 }
 
+template <class T, bool kMask, int L, bool kWalk>
+int launch_lanes(const Rows& a, const Out& o, cudaStream_t s) {
+    const long long per = kRowThreads / L;
+    const unsigned grid = (unsigned)((a.rows + per - 1) / per);
+    if (o.top) lanes_kernel<T, kMask, true, L, kWalk><<<grid, kRowThreads, 0, s>>>(a, o);
+    else lanes_kernel<T, kMask, false, L, kWalk><<<grid, kRowThreads, 0, s>>>(a, o);
+    return (int)cudaGetLastError();
+}
+
+// By the rows' vectors and number alone: a row's sums do not depend on what else is asked for.
+template <class T, bool kMask>
+int launch_rows(const Rows& a, const Out& o, cudaStream_t s) {
+    // the most vectors that a row has
+    const bool even = (uintptr_t)a.logits % 16 == 0 && a.row_stride * (long long)sizeof(T) % 16 == 0;
+    const int nv = (int)(((long long)a.width + Vec<T>::n - 1) / Vec<T>::n) + (even ? 0 : 1);
+    if (nv <= 8) return launch_lanes<T, kMask, 2, false>(a, o, s);
+    if (nv <= 16) return launch_lanes<T, kMask, 4, false>(a, o, s);
+    if (nv <= 32) return launch_lanes<T, kMask, 8, false>(a, o, s);
+    if (nv <= 64) return launch_lanes<T, kMask, 16, false>(a, o, s);
+    if (nv <= 128) return launch_lanes<T, kMask, 32, false>(a, o, s);
+    if (nv <= 1024 && a.rows >= 8 * 148) return launch_lanes<T, kMask, 32, true>(a, o, s);
+    return o.top ? launch_long<T, kMask, true>(a, o, nv, s) : launch_long<T, kMask, false>(a, o, nv, s);
+}
+
 template <class T>
 int launch(const Rows& a, const Out& o, cudaStream_t s) {
-    if (a.width <= kShort) return launch_short<T, 1>(a, o, s);
-    if (a.width <= kShort * 2) return launch_short<T, 2>(a, o, s);
-    if (a.width <= kShort * 4) return launch_short<T, 4>(a, o, s);
-    if (a.width <= kShort * 8) return launch_short<T, 8>(a, o, s);
-    if (a.mask) return o.top ? launch_long<T, true, true>(a, o, s) : launch_long<T, true, false>(a, o, s);
-    return o.top ? launch_long<T, false, true>(a, o, s) : launch_long<T, false, false>(a, o, s);
-}
-
-struct Grad {
-    const float *stats, *entropy, *d_logp, *d_entropy;
-    void* grad;
-    long long grad_stride;
-};
-
-constexpr int kThreads = 256;
-
-template <class T>
-__global__ void __launch_bounds__(kThreads) logprob_grad_kernel(Rows a, Grad b) {
-    const long long row = blockIdx.x;
-    const float m = b.stats[2 * row], logsum = b.stats[2 * row + 1];
-    const float h = b.d_entropy ? b.d_entropy[row] : 0.0f, H = b.d_entropy ? b.entropy[row] : 0.0f;
-    const long long act = action_of(a, row);
-    float g = 0.0f;
-    if (b.d_logp && act >= 0 && act < a.width && logit<T>(a, row, (int)act) != -kInf) g = b.d_logp[row];
-    __syncthreads();  // the action's logit may be what another thread overwrites
-    T* grad = (T*)b.grad + row * b.grad_stride;
-    for (int j = threadIdx.x; j < a.width; j += kThreads) {
-        const float z = logit<T>(a, row, j);
-        float d = 0.0f;
-        if (z != -kInf) {
-            const float lp = fmaxf((z - m) * a.scale - logsum, -1e4f) + (m - m), p = expf(lp);
-            d = -p * (g + h * (lp + H));
-            if (j == act) d += g;
-        }
-        grad[j] = from_float<T>(d * a.scale);
+    if (a.width <= kShort) {
+        short_kernel<T><<<(unsigned)((a.rows + kShortThreads - 1) / kShortThreads), kShortThreads, 0, s>>>(a, o);
+        return (int)cudaGetLastError();
     }
+    return a.mask ? launch_rows<T, true>(a, o, s) : launch_rows<T, false>(a, o, s);
 }
 
-bool rows_ok(const void* logits, int type, long long rows, long long width, long long row_stride,
-             const unsigned char* mask, long long mask_stride, const void* actions, int action_bytes, float scale) {
-    if (type < B3X_F32 || type > B3X_F16 || rows < 0 || rows > 0x7fffffff || !(scale > 0.0f) || !std::isfinite(scale))
-        return false;
-    if (rows == 0) return true;
-    if (width < 1 || width > (1ll << 30) || row_stride < 0 || mask_stride < 0 || !logits) return false;
-    if ((uintptr_t)logits % (type == B3X_F32 ? 4 : 2)) return false;
-    if (actions && action_bytes != 4 && action_bytes != 8) return false;
-    return !actions || (uintptr_t)actions % action_bytes == 0;
-}
 
-bool aligned4(const void* p) { return (uintptr_t)p % 4 == 0; }
 
 }  // namespace
 
@@ -889,24 +783,4 @@ int b3x_train_logprob_gpu(const void* logits, int type, long long rows, long lon
     if (type == B3X_F32) return launch<float>(a, o, (cudaStream_t)stream);
     if (type == B3X_BF16) return launch<__nv_bfloat16>(a, o, (cudaStream_t)stream);
     return launch<__half>(a, o, (cudaStream_t)stream);
-}
-
-int b3x_train_logprob_grad_gpu(const void* logits, int type, long long rows, long long width, long long row_stride,
-        const unsigned char* mask, long long mask_stride, const void* actions, int action_bytes, float scale,
-        const float* stats, const float* entropy, const float* d_logp, const float* d_entropy, void* grad,
-        long long grad_stride, void* stream) {
-    if (!rows_ok(logits, type, rows, width, row_stride, mask, mask_stride, actions, action_bytes, scale))
-        return (int)cudaErrorInvalidValue;
-    if (rows == 0) return (int)cudaSuccess;
-    if (!stats || !grad || (d_logp && !actions) || (d_entropy && !entropy) || !aligned4(stats) || !aligned4(entropy) ||
-        !aligned4(d_logp) || !aligned4(d_entropy) || (uintptr_t)grad % (type == B3X_F32 ? 4 : 2) ||
-        !apart(rows, width, grad_stride, 1) || (grad == logits && rows > 1 && grad_stride != row_stride))
-        return (int)cudaErrorInvalidValue;
-    const Rows a{logits, rows, row_stride, mask, mask_stride, actions, action_bytes, (int)width, scale};
-    const Grad b{stats, entropy, d_logp, d_entropy, grad, grad_stride};
-    const unsigned grid = (unsigned)rows;
-    if (type == B3X_F32) logprob_grad_kernel<float><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a, b);
-    if (type == B3X_BF16) logprob_grad_kernel<__nv_bfloat16><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a, b);
-    if (type == B3X_F16) logprob_grad_kernel<__half><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a, b);
-    return (int)cudaGetLastError();
 }
