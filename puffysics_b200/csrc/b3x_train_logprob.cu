@@ -433,6 +433,7 @@ constexpr int kGroups = 512;         // groups of consecutive vectors whose maxi
 constexpr int kFound = 512;          // logits at or above the threshold that are ranked at once
 constexpr int kMaxWarps = 16;
 constexpr int kMaxCluster = 8;
+constexpr int kSmallWarps = 4, kSmallBlocks = 8;   // of a block where there are many rows
 
 struct Shared {
     Part part[kMaxWarps];
@@ -540,8 +541,8 @@ __device__ __noinline__ void best_groups(Shared& sh, int groups, int top) {
 // registers, or, where the row was walked over, from the groups of 2^shift
 // consecutive vectors whose maxima (kept beside) reach it, which are read again
 // from L2.
-template <class T, bool kMask, bool kTop, bool kOnce>
-__global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, int cluster, int shift) {
+template <class T, bool kMask, bool kTop, bool kOnce, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallBlocks) long_kernel(Rows a, Out o, int cluster, int shift) {
     __shared__ Shared sh;
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
     const int rank = cluster > 1 ? (int)cluster_rank() : 0;
@@ -579,13 +580,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, 
             if (shift >= 7) {
                 const uint32_t key = __reduce_max_sync(~0u, key_of(here));
                 if (lane == 0) atomicMax(&sh.group[(base - v0) >> shift], key);
-            } else if (shift == 6) {   // a group is a warp's vectors of two u
-#pragma unroll
-                for (int u = 0; u < kUnroll; u += 2) {
-                    const uint32_t key = __reduce_max_sync(~0u, key_of(max_nan(top[u], top[u + 1])));
-                    if (lane == 0 && base + u * 32 < v1) sh.group[(base - v0) / 64 + u / 2] = key;
-                }
-            } else {                   // 5: of one u
+            } else {   // 5: a group is a warp's vectors of one u
 #pragma unroll
                 for (int u = 0; u < kUnroll; u++) {
                     const uint32_t key = __reduce_max_sync(~0u, key_of(top[u]));
@@ -640,7 +635,8 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 2) long_kernel(Rows a, Out o, 
                     for (int u = 0; u < kUnroll; u++) {
                         const int k = i + u * blockDim.x;
                         v[u] = k < again ? v0 + (sh.order[k >> shift] << shift) + (k & ((1 << shift) - 1)) : v1;
-                        q[u] = v[u] < v1 ? src.load(v[u]) : no_vector<T>();
+                        if (v[u] >= 2 && v[u] < min(v1, src.last())) q[u] = src.inner(v[u]);
+                        else q[u] = v[u] < v1 ? src.load(v[u]) : no_vector<T>();
                     }
 #pragma unroll
                     for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v[u], threshold);
@@ -714,8 +710,8 @@ int launch_long(const Rows& a, const Out& o, int nv, cudaStream_t s) {
     const int warps = once ? (each + kTile - 1) / kTile : !many ? kMaxWarps : each > 8192 ? 4 : 2;
     int shift = 0;
     if (!once) {
-        shift = each <= 8192 ? 5 : 6;   // some hundred groups
-        while ((each + (1 << shift) - 1) >> shift > kGroups) shift++;
+        shift = 5;   // 32 vectors a group, or 128 and more
+        while ((each + (1 << shift) - 1) >> shift > kGroups) shift = shift == 5 ? 7 : shift + 1;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.rows * cluster));
@@ -727,8 +723,11 @@ int launch_long(const Rows& a, const Out& o, int nv, cudaStream_t s) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    if (once) return (int)cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, true>, a, o, cluster, shift);
-    return (int)cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, false>, a, o, cluster, shift);
+    if (many)
+        return (int)(once ? cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, true, kSmallWarps>, a, o, cluster, shift)
+                          : cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, false, kSmallWarps>, a, o, cluster, shift));
+    return (int)(once ? cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, true, kMaxWarps>, a, o, cluster, shift)
+                      : cudaLaunchKernelEx(&cfg, long_kernel<T, kMask, kTop, false, kMaxWarps>, a, o, cluster, shift));
 }
 
 template <class T, bool kMask, int L, bool kWalk>

@@ -69,7 +69,8 @@ __global__ void __launch_bounds__(kThreads, 2) grad_kernel(const Rows a, const G
 #pragma unroll
         for (int u = 0; u < kUnroll; u++) {
             const int v = base + u * lanes + lane;
-            if (v < nv) q[u] = src.load(v);
+            if (v >= 2 && v < src.last()) q[u] = src.inner(v);
+            else if (v < nv) q[u] = src.load(v);
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; u++) {

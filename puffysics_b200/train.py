@@ -33,6 +33,10 @@ _F32, _BF16, _F16, _E4M3, _U8 = range(5)
 _FLOATS = {torch.float32: _F32, torch.bfloat16: _BF16, torch.float16: _F16}
 _BYTES = {torch.uint8: _U8, torch.bool: _U8}
 
+_Strides = ctypes.c_longlong * 11
+_numel, _dense, _where, _pointer = (torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device,
+                                    torch.Tensor.data_ptr)
+
 _lib = None
 
 
@@ -58,18 +62,25 @@ def lib():
     return _lib
 
 
-def _s(stream):
-    return (torch.cuda.current_stream() if stream is None else stream).cuda_stream
+_device = torch.cuda.current_device
+# the current stream's handle without the object around it, which costs as much as a launch
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _here(t):
-    """Whether a tensor is on the current CUDA device."""
-    return t.is_cuda and t.get_device() == torch.cuda.current_device()
+def _s(stream, device):
+    return _raw_stream(device) if stream is None else stream.cuda_stream
 
 
-def _out(t, shape, dtype=torch.float32):
-    """Whether an optional output has this shape and type, dense."""
-    return t is None or (t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.is_cuda)
+def _vec(t, n, device, dtype=torch.float32):
+    """Whether an optional tensor is a dense one of n elements, of this type, on the device."""
+    return t is None or (t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
+                         and t.get_device() == device)
+
+
+def _mat(t, rows, cols, device, dtype=torch.float32):
+    """The same for (rows, cols)."""
+    return t is None or (t.dtype is dtype and t.shape == (rows, cols) and t.is_contiguous() and t.get_device() == device)
 
 
 def _p(t):
@@ -77,23 +88,27 @@ def _p(t):
 
 
 def _rows(logits, actions, mask):
-    """The leading arguments of the two calls over rows of logits, or None."""
-    if logits.dim() != 2 or logits.dtype not in _FLOATS or not _here(logits):
+    """The leading arguments of the two calls over rows of logits, and the device; or None."""
+    kind = _FLOATS.get(logits.dtype)
+    if kind is None or logits.dim() != 2 or logits.get_device() < 0:
         return None
+    device = _device()
     rows, width = logits.shape
-    if width > 1 and logits.stride(1) != 1:
+    row_stride, stride = logits.stride()
+    if logits.get_device() != device or (stride != 1 and width > 1):
         return None
     mask_stride = action_bytes = 0
     if actions is not None:
-        action_bytes = 8 if actions.dtype is torch.int64 else 4 if actions.dtype is torch.int32 else 0
-        if not action_bytes or actions.shape != (rows,) or not actions.is_contiguous() or not _here(actions):
+        action_bytes = 8 if actions.dtype is torch.int64 else 4
+        if not _vec(actions, rows, device, torch.int64 if action_bytes == 8 else torch.int32):
             return None
     if mask is not None:
-        if mask.dtype not in _BYTES or mask.shape != logits.shape or (width > 1 and mask.stride(1) != 1) or not _here(mask):
+        if mask.dtype not in _BYTES or mask.shape != logits.shape or mask.get_device() != device:
             return None
-        mask_stride = mask.stride(0)
-    return (_p(logits), _FLOATS[logits.dtype], rows, width, logits.stride(0), _p(mask), mask_stride, _p(actions),
-            action_bytes)
+        mask_stride, stride = mask.stride()
+        if stride != 1 and width > 1:
+            return None
+    return (logits.data_ptr(), kind, rows, width, row_stride, _p(mask), mask_stride, _p(actions), action_bytes), device
 
 
 def logprob(logits, actions=None, logp=None, entropy=None, stats=None, top_ids=None, top_logp=None, mask=None,
@@ -111,18 +126,21 @@ def logprob(logits, actions=None, logp=None, entropy=None, stats=None, top_ids=N
     a = _rows(logits, actions, mask)
     if a is None:
         return CUDA_ERROR_INVALID_VALUE
+    a, device = a
     rows = a[2]
     top = 0
     if top_ids is not None or top_logp is not None:
         if top_ids is None or top_logp is None or top_ids.dim() != 2:
             return CUDA_ERROR_INVALID_VALUE
         top = top_ids.shape[1]
-        if not _out(top_ids, (rows, top), torch.int32) or not _out(top_logp, (rows, top)):
+        if not _mat(top_ids, rows, top, device, torch.int32) or not _mat(top_logp, rows, top, device):
             return CUDA_ERROR_INVALID_VALUE
-    if not (_out(logp, (rows,)) and _out(entropy, (rows,)) and _out(stats, (rows, 2))):
+        if top == 0:
+            top_ids = top_logp = None
+    if not (_vec(logp, rows, device) and _vec(entropy, rows, device) and _mat(stats, rows, 2, device)):
         return CUDA_ERROR_INVALID_VALUE
-    return lib().b3x_train_logprob_gpu(*a, scale, _p(logp), _p(entropy), _p(stats), top, _p(top_ids) if top else None,
-                                       _p(top_logp) if top else None, _s(stream))
+    return lib().b3x_train_logprob_gpu(*a, scale, _p(logp), _p(entropy), _p(stats), top, _p(top_ids), _p(top_logp),
+                                       _s(stream, device))
 
 
 def logprob_grad(logits, stats, grad, actions=None, d_logp=None, entropy=None, d_entropy=None, mask=None, scale=1.0,
@@ -134,13 +152,16 @@ def logprob_grad(logits, stats, grad, actions=None, d_logp=None, entropy=None, d
     a = _rows(logits, actions, mask)
     if a is None:
         return CUDA_ERROR_INVALID_VALUE
+    a, device = a
     rows, width = a[2], a[3]
-    if (grad.dtype is not logits.dtype or grad.shape != logits.shape or (width > 1 and grad.stride(1) != 1)
-            or not _here(grad) or not _out(stats, (rows, 2)) or not _out(entropy, (rows,)) or not _out(d_logp, (rows,))
-            or not _out(d_entropy, (rows,))):
+    if grad.dtype is not logits.dtype or grad.shape != logits.shape or grad.get_device() != device:
         return CUDA_ERROR_INVALID_VALUE
-    return lib().b3x_train_logprob_grad_gpu(*a, scale, _p(stats), _p(entropy), _p(d_logp), _p(d_entropy), _p(grad),
-                                            grad.stride(0), _s(stream))
+    grad_stride, stride = grad.stride()
+    if ((stride != 1 and width > 1) or stats is None or not _mat(stats, rows, 2, device)
+            or not _vec(entropy, rows, device) or not _vec(d_logp, rows, device) or not _vec(d_entropy, rows, device)):
+        return CUDA_ERROR_INVALID_VALUE
+    return lib().b3x_train_logprob_grad_gpu(*a, scale, stats.data_ptr(), _p(entropy), _p(d_logp), _p(d_entropy),
+                                            grad.data_ptr(), grad_stride, _s(stream, device))
 
 
 def advantage(rewards, values, terminals, last_values, advantages, returns=None, gamma=0.99, lam=0.95, lengths=None,
@@ -152,36 +173,34 @@ def advantage(rewards, values, terminals, last_values, advantages, returns=None,
     float32, bfloat16 or float16; terminals float32, uint8 or bool; lengths
     (envs,) int32, the steps that each environment has."""
     shape = rewards.shape
-    if (len(shape) != 2 or rewards.dtype is not torch.float32 or values.dtype not in _FLOATS
-            or last_values.dtype is not values.dtype or advantages.dtype is not torch.float32
-            or (terminals.dtype is not torch.float32 and terminals.dtype not in _BYTES)
+    kind, f32, device = _FLOATS.get(values.dtype), torch.float32, rewards.get_device()
+    if (len(shape) != 2 or kind is None or rewards.dtype is not f32 or advantages.dtype is not f32
+            or last_values.dtype is not values.dtype
+            or (terminals.dtype is not f32 and terminals.dtype not in _BYTES)
             or values.shape != shape or terminals.shape != shape or advantages.shape != shape
-            or last_values.shape != shape[1:]
-            or not (_here(rewards) and _here(values) and _here(terminals) and _here(last_values) and _here(advantages))):
+            or last_values.shape != shape[1:] or device < 0 or device != _device()
+            or values.get_device() != device or terminals.get_device() != device
+            or last_values.get_device() != device or advantages.get_device() != device):
         return CUDA_ERROR_INVALID_VALUE
-    if returns is not None and (returns.dtype is not torch.float32 or returns.shape != shape or not _here(returns)):
+    if returns is not None and (returns.dtype is not f32 or returns.shape != shape or returns.get_device() != device):
         return CUDA_ERROR_INVALID_VALUE
-    if lengths is not None and (lengths.dtype is not torch.int32 or lengths.shape != shape[1:]
-                                or not lengths.is_contiguous() or not _here(lengths)):
+    if not _vec(lengths, shape[1], device, torch.int32):
         return CUDA_ERROR_INVALID_VALUE
-    strides = (ctypes.c_longlong * 11)(*rewards.stride(), *values.stride(), *terminals.stride(), *last_values.stride(),
-                                       *advantages.stride(), *((0, 0) if returns is None else returns.stride()))
-    return lib().b3x_train_advantage_gpu(shape[0], shape[1], _p(rewards), _p(values), _FLOATS[values.dtype],
-                                         _p(terminals), _F32 if terminals.dtype is torch.float32 else _U8,
-                                         _p(last_values), _p(lengths), _p(advantages), _p(returns), strides, gamma, lam,
-                                         _s(stream))
+    strides = _Strides(*rewards.stride(), *values.stride(), *terminals.stride(), *last_values.stride(),
+                       *advantages.stride(), *((0, 0) if returns is None else returns.stride()))
+    return lib().b3x_train_advantage_gpu(shape[0], shape[1], rewards.data_ptr(), values.data_ptr(), kind,
+                                         terminals.data_ptr(), _F32 if terminals.dtype is f32 else _U8,
+                                         last_values.data_ptr(), _p(lengths), advantages.data_ptr(), _p(returns), strides,
+                                         gamma, lam, _s(stream, device))
 
 
-def _list(tensors, sizes, dtype):
-    """Pointers of a list of dense tensors on the current device, of one type
-    and these element counts; None where they are not."""
-    if len(tensors) != len(sizes):
+def _list(tensors, sizes, dtype, device):
+    """Pointers of a list of dense tensors on the device, of one type and these
+    element counts; None where they are not."""
+    if (list(map(_numel, tensors)) != sizes or not all(map(_dense, tensors)) or any(t.dtype is not dtype for t in tensors)
+            or any(map(device.__ne__, map(_where, tensors)))):
         return None
-    device = torch.cuda.current_device()
-    for t, n in zip(tensors, sizes):
-        if t.dtype is not dtype or t.numel() != n or not t.is_contiguous() or t.get_device() != device:
-            return None
-    return array.array("Q", [t.data_ptr() for t in tensors])
+    return array.array("Q", map(_pointer, tensors))
 
 
 def _addr(a):
@@ -196,14 +215,16 @@ def grad_norm(grads, max_norm, out, workspace, stream=None):
     """Global 2-norm of a list of gradients into out[0], and the factor that
     clips them to max_norm into out[1] (out (2,) float32; NaN where the norm is
     not finite).  workspace: a uint8 tensor of grad_norm_workspace_bytes()."""
-    sizes = array.array("q", [t.numel() for t in grads])
+    device = _device()
+    sizes = list(map(_numel, grads))
     dtype = grads[0].dtype if grads else torch.float32
-    g = _list(grads, sizes, dtype) if dtype in _FLOATS else None
-    if (g is None or not _out(out, (2,)) or out is None or not _here(out) or workspace.dtype is not torch.uint8
-            or not workspace.is_contiguous() or not _here(workspace)):
+    g = _list(grads, sizes, dtype, device) if dtype in _FLOATS else None
+    if (g is None or out is None or not _vec(out, 2, device) or workspace.dtype is not torch.uint8
+            or not workspace.is_contiguous() or workspace.get_device() != device):
         return CUDA_ERROR_INVALID_VALUE
-    return lib().b3x_train_grad_norm_gpu(len(grads), _addr(g), _FLOATS[dtype], _addr(sizes), max_norm, _p(out),
-                                         _p(workspace), workspace.numel(), _s(stream))
+    counts = array.array("q", sizes)   # named, so that it outlives the call
+    return lib().b3x_train_grad_norm_gpu(len(sizes), _addr(g), _FLOATS[dtype], _addr(counts), max_norm,
+                                         out.data_ptr(), workspace.data_ptr(), workspace.numel(), _s(stream, device))
 
 
 def adamw(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
@@ -224,19 +245,20 @@ def adamw(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2=0.999, 
     pt, gt, st = params[0].dtype, grads[0].dtype if len(grads) else None, exp_avg[0].dtype if len(exp_avg) else None
     if pt not in (torch.float32, torch.bfloat16) or gt not in _FLOATS or st not in (torch.float32, torch.float8_e4m3fn):
         return CUDA_ERROR_INVALID_VALUE
-    sizes = array.array("q", [t.numel() for t in params])
-    p, g = _list(params, sizes, pt), _list(grads, sizes, gt)
-    m, v = _list(exp_avg, sizes, st), _list(exp_avg_sq, sizes, st)
+    device = _device()
+    sizes = list(map(_numel, params))
+    p, g = _list(params, sizes, pt, device), _list(grads, sizes, gt, device)
+    m, v = _list(exp_avg, sizes, st, device), _list(exp_avg_sq, sizes, st, device)
     f8 = st is torch.float8_e4m3fn
     if p is None or g is None or m is None or v is None or f8 != (scales is not None):
         return CUDA_ERROR_INVALID_VALUE
     s = c = decays = None
     if f8:
-        s = _list(scales, [(k + BLOCK - 1) // BLOCK * 2 for k in sizes], torch.float32)
+        s = _list(scales, [(k + BLOCK - 1) // BLOCK * 2 for k in sizes], torch.float32, device)
         if s is None:
             return CUDA_ERROR_INVALID_VALUE
     if copies is not None:
-        c = _list(copies, sizes, torch.bfloat16)
+        c = _list(copies, sizes, torch.bfloat16, device)
         if c is None:
             return CUDA_ERROR_INVALID_VALUE
     if isinstance(weight_decay, (list, tuple)):
@@ -244,9 +266,10 @@ def adamw(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2=0.999, 
             return CUDA_ERROR_INVALID_VALUE
         decays, weight_decay = array.array("f", weight_decay), 0.0
     if grad_scale is not None and (grad_scale.dtype is not torch.float32 or grad_scale.numel() != 1
-                                   or not _here(grad_scale)):
+                                   or grad_scale.get_device() != device):
         return CUDA_ERROR_INVALID_VALUE
+    counts = array.array("q", sizes)
     return lib().b3x_train_adamw_gpu(n, _addr(p), _FLOATS[pt], _addr(g), _FLOATS[gt], _addr(m), _addr(v), _addr(s),
-                                     _E4M3 if f8 else _F32, _addr(c), _addr(sizes), _addr(decays), step, lr, beta1,
+                                     _E4M3 if f8 else _F32, _addr(c), _addr(counts), _addr(decays), step, lr, beta1,
                                      beta2, eps, weight_decay, _p(grad_scale), seed is not None,
-                                     (seed or 0) & 0xFFFFFFFF, _s(stream))
+                                     (seed or 0) & 0xFFFFFFFF, _s(stream, device))
