@@ -217,6 +217,8 @@ __device__ __forceinline__ float remote_float(const void* p, unsigned rank) {
 }
 
 constexpr int kMaxThreads = 1024;
+constexpr int kBlockSteps = 8;   // steps a thread
+
 constexpr int kMaxCluster = 8;
 
 struct Shared {
@@ -225,12 +227,13 @@ struct Shared {
 };
 
 // 2^env_bits environments a block, neighbouring lanes neighbouring environments,
-// kSteps steps a thread; a cluster's blocks divide the time.  Long times take
+// kBlockSteps steps a thread; a cluster's blocks divide the time.  Long times take
 // several turns of the block, from the last steps to the first, each with what
 // the one before carried; the blocks of a cluster go through their part once
 // before, for its pair alone (their second reading comes from L2).
-template <class V, class D, int kSteps, bool kVec>
+template <class V, class D, bool kVec>
 __global__ void __launch_bounds__(kMaxThreads) advantage_kernel(const Rollout a, int env_bits, int cluster) {
+    constexpr int kSteps = kBlockSteps;
     __shared__ Shared sh;
     const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int nx = 1 << env_bits, e = threadIdx.x & (nx - 1), seg = threadIdx.x >> env_bits;
@@ -289,22 +292,21 @@ int launch(const Rollout& a, bool vec, cudaStream_t s) {
         advantage_rows_kernel<V, D><<<(unsigned)blocks, kRowThreads, 0, s>>>(a, group, lead);
         return (int)cudaGetLastError();
     }
-    const int steps = vec ? 4 : 8;
     // environments side by side where they are neighbours in memory, fewer while that leaves SMs idle and takes turns
     int bits = 0;
     if (!vec && (a.rt != 1 || a.steps == 1 || a.rn < a.rt)) {
         while (bits < 5 && (1 << bits) < a.envs) bits++;
-        while (bits > 0 && ((a.envs + (1 << bits) - 1) >> bits) < 148 && a.steps > (kMaxThreads >> bits) * steps) bits--;
+        while (bits > 0 && ((a.envs + (1 << bits) - 1) >> bits) < 148 && a.steps > (kMaxThreads >> bits) * kBlockSteps) bits--;
     }
     const long long groups = ((long long)a.envs + (1 << bits) - 1) >> bits;
-    // Threads for all steps, as many as suit (1,024 environments of 8,191 steps one after the other: 54 us with 512, 44
-    // with 256, 39 with 128; 256 steps of 16,384 environments side by side: 20, 18, 22); all where blocks are few, and
+    // Threads for all steps, as many as suit (1,024 environments of 8,191 steps one after the other: 75 us with 512, 64
+    // with 256, 34 with 128; 256 steps of 16,384 environments side by side: 20, 18, 22); all where blocks are few, and
     // clusters then.
     const int most = groups < 148 ? kMaxThreads : vec ? 128 : 256;
     int threads = 32;
-    while (threads < most && (threads >> bits) * steps < need) threads *= 2;
+    while (threads < most && (threads >> bits) * kBlockSteps < need) threads *= 2;
     int cluster = 1;
-    while (cluster < kMaxCluster && groups * cluster * 2 <= 148 && (long long)(threads >> bits) * steps * cluster < need) cluster *= 2;
+    while (cluster < kMaxCluster && groups * cluster * 2 <= 148 && (long long)(threads >> bits) * kBlockSteps * cluster < need) cluster *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(groups * cluster));
     cfg.blockDim = dim3(threads);
@@ -315,8 +317,8 @@ int launch(const Rollout& a, bool vec, cudaStream_t s) {
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    if (vec) return (int)cudaLaunchKernelEx(&cfg, advantage_kernel<V, D, 4, true>, a, bits, cluster);
-    return (int)cudaLaunchKernelEx(&cfg, advantage_kernel<V, D, 8, false>, a, bits, cluster);
+    if (vec) return (int)cudaLaunchKernelEx(&cfg, advantage_kernel<V, D, true>, a, bits, cluster);
+    return (int)cudaLaunchKernelEx(&cfg, advantage_kernel<V, D, false>, a, bits, cluster);
 }
 
 }  // namespace

@@ -99,14 +99,26 @@ struct Row {
     }
 };
 
+// A row's action, read ahead of the sums.
+struct Action {
+    bool any;
+    float z;
+};
 template <class T>
-__device__ __forceinline__ void write_row(const Rows& a, const Out& o, long long row, const Row& r) {
-    if (o.stats) o.stats[2 * row] = r.m, o.stats[2 * row + 1] = r.logsum;
-    if (o.entropy) o.entropy[row] = r.entropy;
+__device__ __forceinline__ Action load_action(const Rows& a, const Out& o, long long row) {
+    Action got{false, 0.0f};
     if (o.logp) {
         const long long j = action_of(a, row);
-        o.logp[row] = j >= 0 && j < a.width ? r.logp(logit<T>(a, row, (int)j), a.scale) : 0.0f;
+        got.any = j >= 0 && j < a.width;
+        if (got.any) got.z = logit<T>(a, row, (int)j);
     }
+    return got;
+}
+
+__device__ __forceinline__ void write_row(const Rows& a, const Out& o, long long row, const Row& r, Action act) {
+    if (o.stats) o.stats[2 * row] = r.m, o.stats[2 * row + 1] = r.logsum;
+    if (o.entropy) o.entropy[row] = r.entropy;
+    if (o.logp) o.logp[row] = act.any ? r.logp(act.z, a.scale) : 0.0f;
 }
 
 __device__ __forceinline__ void write_top(const Out& o, long long row, int k, uint64_t e, const Row& r, float scale) {
@@ -124,6 +136,7 @@ template <class T>
 __global__ void __launch_bounds__(kShortThreads) short_kernel(Rows a, Out o) {
     const long long row = (long long)blockIdx.x * kShortThreads + threadIdx.x;
     if (row >= a.rows) return;
+    const Action act = load_action<T>(a, o, row);
     float z[kShort];
     Part p{-kInf, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -139,7 +152,7 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(Rows a, Out o) {
         p.t = __fmaf_rn(e, x, p.t);
     }
     const Row r = Row::about_maximum(p);
-    write_row<T>(a, o, row, r);
+    write_row(a, o, row, r, act);
     uint64_t last = ~0ull;
     for (int k = 0; k < o.top; k++) {
         uint64_t best = 0;
@@ -294,6 +307,8 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 3 : 4) lanes_kernel(Rows a
     const int nv = on ? src.vectors() : 0;
     const float c = a.scale * kLog2e;
     if (kTop && lane == 0) found[here] = 0;
+    Action act{false, 0.0f};
+    if (on && lane == 0) act = load_action<T>(a, o, row);
     uint4 q[U];
     const auto load = [&](int base) {
 #pragma unroll
@@ -343,8 +358,21 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 3 : 4) lanes_kernel(Rows a
         if (far) p.s = s, p.t = t;
     }
     const Row r = far ? Row::about_maximum(p) : Row(p, c);
-    if (on && lane == 0) write_row<T>(a, o, row, r);
+    if (on && lane == 0) write_row(a, o, row, r, act);
     if (!kTop) return;
+
+    if (!kWalk && o.top == 1 && __all_sync(~0u, p.m == p.m)) {   // the first place of the maximum
+        int first = 0x7FFFFFFF;
+#pragma unroll
+        for (int u = U - 1; u >= 0; u--)
+#pragma unroll
+            for (int n = N - 1; n >= 0; n--)
+                if (element<T>(q[u], n) == p.m) first = (u * L + lane) * N - src.head + n;
+#pragma unroll
+        for (int k = L / 2; k; k /= 2) first = min(first, __shfl_xor_sync(~0u, first, k));
+        if (on && lane == 0) write_top(o, row, 0, p.m == -kInf ? 0 : entry_of(key_of(p.m), first), r, a.scale);
+        return;
+    }
 
     float z;
     if (L == 32) {
@@ -559,6 +587,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallB
         __syncthreads();
     }
 
+    Action act{false, 0.0f};
+    if (threadIdx.x == 0 && rank == 0) act = load_action<T>(a, o, row);
     uint4 q[kUnroll];
     Part p = empty_part();
     for (int base = v0 + warp * kTile; base < v1 || kOnce; base += warps * kTile) {
@@ -690,7 +720,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallB
         for (int w = 0; w < warps; w++) p.s += sh.far[w].x, p.t += sh.far[w].y;
     }
     const Row r = far ? Row::about_maximum(p) : Row(p, c);
-    if (threadIdx.x == 0) write_row<T>(a, o, row, r);
+    if (threadIdx.x == 0) write_row(a, o, row, r, act);
     if (kTop)
         for (int k = threadIdx.x; k < o.top; k += blockDim.x) write_top(o, row, k, sh.list[k], r, a.scale);
 }
