@@ -141,6 +141,13 @@ __device__ __forceinline__ uint64_t sqrt2(uint64_t v) {
     return fma2(fma2(minus, s, v), half, s);
 }
 
+// The least of three numbers, NaN below all.
+__device__ __forceinline__ float least3(float a, float b, float c) {
+    float y;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
 // The largest of a warp's numbers that are not negative; NaN is the largest.
 __device__ __forceinline__ float warp_most(float x) {
     return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(x) & 0x7FFFFFFFu));
@@ -150,6 +157,212 @@ __device__ __forceinline__ float warp_most(float x) {
 // so that every load and store is a whole line however wide its type.  The
 // moments' operations round one by one: their codes are those of the plain
 // formula, bit for bit.
+template <class P, class G, bool kF8, bool kRandom, bool kWhole>
+__device__ __forceinline__ void update(const Tensor& t, const Hyper& h, const float gs, const long long base, const int lane) {
+    const long long n = t.n;
+    P* const pp = (P*)t.p;
+    const G* const pg = (const G*)t.g;
+    float p[2][4], g[2][4], m[2][4], v[2][4];
+    uint32_t cm[2], cv[2];
+    float sm = 0.0f, sr = 0.0f;
+    if (kF8) {
+        const float2 s = *reinterpret_cast<const float2*>(t.scales + base / 256 * 2);
+        sm = s.x, sr = s.y;
+    }
+    if (kWhole) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const long long i = base + k * 128 + lane * 4;
+            load4(g[k], pg + i);
+            load4(p[k], pp + i);
+            if (kF8) {
+                cm[k] = __ldcs(reinterpret_cast<const uint32_t*>((const unsigned char*)t.m + i));
+                cv[k] = __ldcs(reinterpret_cast<const uint32_t*>((const unsigned char*)t.v + i));
+            } else {
+                load4(m[k], (const float*)t.m + i);
+                load4(v[k], (const float*)t.v + i);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            cm[k] = cv[k] = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const long long i = base + k * 128 + lane * 4 + j;
+                const bool in = i < n;
+                g[k][j] = in ? to_float(pg[i]) : 0.0f;
+                p[k][j] = in ? to_float(pp[i]) : 0.0f;
+                if (kF8) {
+                    cm[k] |= in ? (uint32_t)((const unsigned char*)t.m)[i] << j * 8 : 0u;
+                    cv[k] |= in ? (uint32_t)((const unsigned char*)t.v)[i] << j * 8 : 0u;
+                } else {
+                    m[k][j] = in ? ((const float*)t.m)[i] : 0.0f;
+                    v[k][j] = in ? ((const float*)t.v)[i] : 0.0f;
+                }
+            }
+        }
+    }
+    float most_m = 0.0f, most_r = 0.0f, most_p = 0.0f;
+    const uint64_t gs2 = pack2(gs, gs), sm2 = pack2(sm, sm), sr2 = pack2(sr, sr), b1 = pack2(h.b1, h.b1), c1 = pack2(h.c1, h.c1),
+                   b2 = pack2(h.b2, h.b2), c2 = pack2(h.c2, h.c2), root = pack2(h.root, h.root), eps = pack2(h.eps, h.eps),
+                   keep = pack2(t.keep, t.keep), rate = pack2(-h.rate, -h.rate);
+    float least_v = kInf, most_v = 0.0f;
+    uint64_t m2[4], v2[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int k = q / 2, j = q % 2 * 2;
+        if (kF8) {
+            const float2 a = decode2(cm[k] >> j * 8), b = decode2(cv[k] >> j * 8);
+            m2[q] = mul2(pack2(a.x, a.y), sm2);
+            const uint64_t r = mul2(pack2(b.x, b.y), sr2);
+            v2[q] = mul2(r, r);
+        } else {
+            m2[q] = pack2(m[k][j], m[k][j + 1]);
+            v2[q] = pack2(v[k][j], v[k][j + 1]);
+        }
+        const uint64_t x = mul2(pack2(g[k][j], g[k][j + 1]), gs2);
+        m2[q] = sum2(mul2(m2[q], b1), mul2(x, c1));
+        v2[q] = sum2(mul2(v2[q], b2), mul2(mul2(x, x), c2));
+        const float2 vv = unpack2(v2[q]);
+        least_v = least3(least_v, vv.x, vv.y), most_v = most3(most_v, vv.x, vv.y);
+    }
+    const bool usual = least_v >= 0x1p-96f && most_v <= 0x1p100f;
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int k = q / 2, j = q % 2 * 2;
+        const float2 vv = unpack2(v2[q]), nm = unpack2(m2[q]);
+        float2 r = unpack2(sqrt2(v2[q]));
+        if (!usual) r = make_float2(sqrtf(vv.x), sqrtf(vv.y));
+        const float2 d = unpack2(fma2(pack2(r.x, r.y), root, eps));
+        const uint64_t step = mul2(mul2(m2[q], pack2(reciprocal(d.x), reciprocal(d.y))), rate);
+        const float2 np = unpack2(fma2(pack2(p[k][j], p[k][j + 1]), keep, step));
+        p[k][j] = np.x, p[k][j + 1] = np.y;
+        m[k][j] = nm.x, m[k][j + 1] = nm.y;
+        if (kF8) {
+            most_m = most3(most_m, nm.x, nm.y), most_r = most3(most_r, r.x, r.y);
+            v[k][j] = r.x, v[k][j + 1] = r.y;
+        } else {
+            v[k][j] = vv.x, v[k][j + 1] = vv.y;
+        }
+        if (kRandom && sizeof(P) == 2) most_p = most3(most_p, np.x, np.y);
+    }
+    if (!kF8) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const long long i = base + k * 128 + lane * 4;
+            if (kWhole) {
+                store4((float*)t.m + i, m[k]);
+                store4((float*)t.v + i, v[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (i + j < n) ((float*)t.m)[i + j] = m[k][j], ((float*)t.v)[i + j] = v[k][j];
+            }
+        }
+    }
+    if (t.copy) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const long long i = base + k * 128 + lane * 4;
+            if (kWhole) {
+                store4(t.copy + i, p[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (i + j < n) t.copy[i + j] = __float2bfloat16_rn(p[k][j]);
+            }
+        }
+    }
+    uint32_t bits[2][4];
+    if (kRandom) {
+        const uint32_t at = (uint32_t)(base + lane * 4) * 0x9E3779B1u + (uint32_t)(base >> 32) * 0x6A09E667u + t.key;
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) bits[k][j] = mix(at + (k * 128 + j) * 0x9E3779B1u);
+    }
+    if (kRandom && sizeof(P) == 2) {
+        uint32_t low[2][4];
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) low[k][j] = mix(bits[k][j] + 0x9E3779B1u) & 0xFFFFu;
+        if (most_p != most_p) {   // NaN stays what it is
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (p[k][j] != p[k][j]) low[k][j] = 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const long long i = base + k * 128 + lane * 4;
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j] = __float_as_uint(p[k][j]) + low[k][j];
+            const uint2 q = make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
+            if (kWhole) {
+                __stcs(reinterpret_cast<uint2*>(pp + i), q);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (i + j < n) reinterpret_cast<uint16_t*>(pp)[i + j] = (uint16_t)(w[j] >> 16);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const long long i = base + k * 128 + lane * 4;
+            if (kWhole) {
+                store4(pp + i, p[k]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (i + j < n) pp[i + j] = from_float<P>(p[k][j]);
+            }
+        }
+    }
+    if (!kF8) return;
+    most_m = warp_most(most_m), most_r = warp_most(most_r);
+    // a division for each quarter of the lanes: the scales, and what makes codes of the moments
+    const float most = lane < 16 ? most_m : most_r;
+    const float part = most < 0x1p-100f ? 0.0f : lane & 8 ? 448.0f / most : most / 448.0f;
+    if ((lane & 15) == 0) t.scales[base / 256 * 2 + lane / 16] = part;
+    const float im = __shfl_sync(~0u, part, 8), ir = __shfl_sync(~0u, part, 24);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        uint32_t wm[4], wv[4], sign[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            wm[j] = encode<kRandom>(m[k][j] * im, bits[k][j] << 4);
+            wv[j] = encode<kRandom>(v[k][j] * ir, bits[k][j] >> 12);
+            sign[j] = __float_as_uint(m[k][j]);
+        }
+        cm[k] = upper_bytes(wm) | (upper_bytes(sign) & 0x80808080u);
+        cv[k] = upper_bytes(wv);
+        // a moment above zero never becomes zero: it would divide by eps alone
+        if (((cv[k] + 0x7F7F7F7Fu) & 0x80808080u) != 0x80808080u && ir != 0.0f) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (v[k][j] > 0.0f && !(cv[k] >> j * 8 & 0xFFu)) cv[k] |= 1u << j * 8;
+        }
+        const long long i = base + k * 128 + lane * 4;
+        if (kWhole) {
+            __stcs(reinterpret_cast<uint32_t*>((unsigned char*)t.m + i), cm[k]);
+            __stcs(reinterpret_cast<uint32_t*>((unsigned char*)t.v + i), cv[k]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i + j < n) {
+                    ((unsigned char*)t.m)[i + j] = (unsigned char)(cm[k] >> j * 8);
+                    ((unsigned char*)t.v)[i + j] = (unsigned char)(cv[k] >> j * 8);
+                }
+        }
+    }
+}
+
+// kWhole: all 256 elements, every array at a multiple of 4 of them.
 template <class P, class G, bool kF8, bool kRandom, int N>
 __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ List<N> list, const Hyper h) {
     const float gs = h.grad_scale ? *h.grad_scale : 1.0f;
@@ -158,203 +371,9 @@ __global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constan
     const Tensor& t = list.t[which];
     const int lane = threadIdx.x % 32;
     long long base = ((long long)(blockIdx.x - list.first[which]) * list.turns * (kTurn / 256) + threadIdx.x / 32) * 256;
-    const long long n = t.n;
-    P* const pp = (P*)t.p;
-    const G* const pg = (const G*)t.g;
-    for (int turn = 0; turn < list.turns && base < n; turn++, base += kTurn) {
-        const bool whole = t.even && base + 256 <= n;
-        float p[2][4], g[2][4], m[2][4], v[2][4];
-        uint32_t cm[2], cv[2];
-        float sm = 0.0f, sr = 0.0f;
-        if (kF8) {
-            const float2 s = *reinterpret_cast<const float2*>(t.scales + base / 256 * 2);
-            sm = s.x, sr = s.y;
-        }
-        if (whole) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const long long i = base + k * 128 + lane * 4;
-                load4(g[k], pg + i);
-                load4(p[k], pp + i);
-                if (kF8) {
-                    cm[k] = __ldcs(reinterpret_cast<const uint32_t*>((const unsigned char*)t.m + i));
-                    cv[k] = __ldcs(reinterpret_cast<const uint32_t*>((const unsigned char*)t.v + i));
-                } else {
-                    load4(m[k], (const float*)t.m + i);
-                    load4(v[k], (const float*)t.v + i);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                cm[k] = cv[k] = 0;
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const long long i = base + k * 128 + lane * 4 + j;
-                    const bool in = i < n;
-                    g[k][j] = in ? to_float(pg[i]) : 0.0f;
-                    p[k][j] = in ? to_float(pp[i]) : 0.0f;
-                    if (kF8) {
-                        cm[k] |= in ? (uint32_t)((const unsigned char*)t.m)[i] << j * 8 : 0u;
-                        cv[k] |= in ? (uint32_t)((const unsigned char*)t.v)[i] << j * 8 : 0u;
-                    } else {
-                        m[k][j] = in ? ((const float*)t.m)[i] : 0.0f;
-                        v[k][j] = in ? ((const float*)t.v)[i] : 0.0f;
-                    }
-                }
-            }
-        }
-        float most_m = 0.0f, most_r = 0.0f, most_p = 0.0f;
-        const uint64_t gs2 = pack2(gs, gs), sm2 = pack2(sm, sm), sr2 = pack2(sr, sr), b1 = pack2(h.b1, h.b1),
-                       c1 = pack2(h.c1, h.c1), b2 = pack2(h.b2, h.b2), c2 = pack2(h.c2, h.c2), root = pack2(h.root, h.root),
-                       eps = pack2(h.eps, h.eps), keep = pack2(t.keep, t.keep), rate = pack2(-h.rate, -h.rate);
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-                uint64_t m2, v2;
-                if (kF8) {
-                    const float2 a = decode2(cm[k] >> j * 8), b = decode2(cv[k] >> j * 8);
-                    m2 = mul2(pack2(a.x, a.y), sm2);
-                    const uint64_t r = mul2(pack2(b.x, b.y), sr2);
-                    v2 = mul2(r, r);
-                } else {
-                    m2 = pack2(m[k][j], m[k][j + 1]);
-                    v2 = pack2(v[k][j], v[k][j + 1]);
-                }
-                const uint64_t x = mul2(pack2(g[k][j], g[k][j + 1]), gs2);
-                m2 = sum2(mul2(m2, b1), mul2(x, c1));
-                v2 = sum2(mul2(v2, b2), mul2(mul2(x, x), c2));
-                const float2 vv = unpack2(v2);
-                float2 r;
-                if (fminf(vv.x, vv.y) >= 0x1p-96f && fmaxf(vv.x, vv.y) <= 0x1p100f) r = unpack2(sqrt2(v2));
-                else r = make_float2(sqrtf(vv.x), sqrtf(vv.y));
-                const float2 d = unpack2(fma2(pack2(r.x, r.y), root, eps));
-                const uint64_t step = mul2(mul2(m2, pack2(reciprocal(d.x), reciprocal(d.y))), rate);
-                const float2 np = unpack2(fma2(pack2(p[k][j], p[k][j + 1]), keep, step)), nm = unpack2(m2);
-                p[k][j] = np.x, p[k][j + 1] = np.y;
-                m[k][j] = nm.x, m[k][j + 1] = nm.y;
-                if (kF8) {
-                    most_m = most3(most_m, nm.x, nm.y), most_r = most3(most_r, r.x, r.y);
-                    v[k][j] = r.x, v[k][j + 1] = r.y;
-                } else {
-                    v[k][j] = vv.x, v[k][j + 1] = vv.y;
-                }
-                if (kRandom && sizeof(P) == 2) most_p = most3(most_p, np.x, np.y);
-            }
-        if (!kF8) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const long long i = base + k * 128 + lane * 4;
-                if (whole) {
-                    store4((float*)t.m + i, m[k]);
-                    store4((float*)t.v + i, v[k]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (i + j < n) ((float*)t.m)[i + j] = m[k][j], ((float*)t.v)[i + j] = v[k][j];
-                }
-            }
-        }
-        if (t.copy) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const long long i = base + k * 128 + lane * 4;
-                if (whole) {
-                    store4(t.copy + i, p[k]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (i + j < n) t.copy[i + j] = __float2bfloat16_rn(p[k][j]);
-                }
-            }
-        }
-        uint32_t bits[2][4];
-        if (kRandom) {
-            const uint32_t at = (uint32_t)(base + lane * 4) * 0x9E3779B1u + (uint32_t)(base >> 32) * 0x6A09E667u + t.key;
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) bits[k][j] = mix(at + (k * 128 + j) * 0x9E3779B1u);
-        }
-        if (kRandom && sizeof(P) == 2) {
-            uint32_t low[2][4];
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) low[k][j] = mix(bits[k][j] + 0x9E3779B1u) & 0xFFFFu;
-            if (most_p != most_p) {   // NaN stays what it is
-#pragma unroll
-                for (int k = 0; k < 2; k++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (p[k][j] != p[k][j]) low[k][j] = 0;
-            }
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const long long i = base + k * 128 + lane * 4;
-                uint32_t w[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) w[j] = __float_as_uint(p[k][j]) + low[k][j];
-                const uint2 q = make_uint2(__byte_perm(w[0], w[1], 0x7632), __byte_perm(w[2], w[3], 0x7632));
-                if (whole) {
-                    __stcs(reinterpret_cast<uint2*>(pp + i), q);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (i + j < n) reinterpret_cast<uint16_t*>(pp)[i + j] = (uint16_t)(w[j] >> 16);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const long long i = base + k * 128 + lane * 4;
-                if (whole) {
-                    store4(pp + i, p[k]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (i + j < n) pp[i + j] = from_float<P>(p[k][j]);
-                }
-            }
-        }
-        if (!kF8) continue;
-        most_m = warp_most(most_m), most_r = warp_most(most_r);
-        // a division for each quarter of the lanes: the scales, and what makes codes of the moments
-        const float most = lane < 16 ? most_m : most_r;
-        const float part = most < 0x1p-100f ? 0.0f : lane & 8 ? 448.0f / most : most / 448.0f;
-        if ((lane & 15) == 0) t.scales[base / 256 * 2 + lane / 16] = part;
-        const float im = __shfl_sync(~0u, part, 8), ir = __shfl_sync(~0u, part, 24);
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            uint32_t wm[4], wv[4], sign[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                wm[j] = encode<kRandom>(m[k][j] * im, bits[k][j] << 4);
-                wv[j] = encode<kRandom>(v[k][j] * ir, bits[k][j] >> 12);
-                sign[j] = __float_as_uint(m[k][j]);
-            }
-            cm[k] = upper_bytes(wm) | (upper_bytes(sign) & 0x80808080u);
-            cv[k] = upper_bytes(wv);
-            // a moment above zero never becomes zero: it would divide by eps alone
-            if (((cv[k] + 0x7F7F7F7Fu) & 0x80808080u) != 0x80808080u && ir != 0.0f) {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (v[k][j] > 0.0f && !(cv[k] >> j * 8 & 0xFFu)) cv[k] |= 1u << j * 8;
-            }
-            const long long i = base + k * 128 + lane * 4;
-            if (whole) {
-                __stcs(reinterpret_cast<uint32_t*>((unsigned char*)t.m + i), cm[k]);
-                __stcs(reinterpret_cast<uint32_t*>((unsigned char*)t.v + i), cv[k]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (i + j < n) {
-                        ((unsigned char*)t.m)[i + j] = (unsigned char)(cm[k] >> j * 8);
-                        ((unsigned char*)t.v)[i + j] = (unsigned char)(cv[k] >> j * 8);
-                    }
-            }
-        }
+    for (int turn = 0; turn < list.turns && base < t.n; turn++, base += kTurn) {
+        if (t.even && base + 256 <= t.n) update<P, G, kF8, kRandom, true>(t, h, gs, base, lane);
+        else update<P, G, kF8, kRandom, false>(t, h, gs, base, lane);
     }
 }
 
