@@ -7,7 +7,7 @@ Each iteration rolls the batch out for 64 steps (puffysics_b200/hover_env.py
 writes rewards and terminals into the rollout's rows, train.logprob the log
 probability of each action), turns rewards and terminals into advantages and
 returns (train.advantage), and goes over the rollout a few times in shuffled
-quarters: a clipped surrogate of the new and old log probabilities with an
+eighths: a clipped surrogate of the new and old log probabilities with an
 entropy bonus, whose derivatives train.logprob_grad turns into gradients of the
 logits, torch's backward pass through the network's two layers, a clip of the
 gradients' norm (train.grad_norm) and a step (train.adamw), with moments in 32
@@ -63,7 +63,7 @@ class AdamW:
                           grad_scale=self.norm[1:], seed=1 if self.scales else None))
 
 
-def run(envs=4096, iterations=40, steps=64, epochs=3, parts=4, lr=3e-3, clip=0.2, bonus=0.003, eight_bit=False, seed=1,
+def run(envs=4096, iterations=40, steps=64, epochs=3, parts=8, lr=1e-3, clip=0.2, bonus=0.003, eight_bit=False, seed=1,
         report=None):
     """Mean reward a step of each iteration's rollout."""
     build.build()

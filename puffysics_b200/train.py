@@ -72,43 +72,53 @@ def _s(stream, device):
     return _raw_stream(device) if stream is None else stream.cuda_stream
 
 
+class _Refused(Exception):
+    """An argument that a call does not take: the call returns cudaErrorInvalidValue."""
+
+
 def _vec(t, n, device, dtype=torch.float32):
-    """Whether an optional tensor is a dense one of n elements, of this type, on the device."""
-    return t is None or (t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous()
-                         and t.get_device() == device)
+    """The pointer of a dense tensor of n elements, of this type, on the device; None for none."""
+    if t is None:
+        return None
+    if t.dtype is dtype and t.dim() == 1 and t.numel() == n and t.is_contiguous() and t.get_device() == device:
+        return t.data_ptr()
+    raise _Refused
 
 
 def _mat(t, rows, cols, device, dtype=torch.float32):
     """The same for (rows, cols)."""
-    return t is None or (t.dtype is dtype and t.shape == (rows, cols) and t.is_contiguous() and t.get_device() == device)
-
-
-def _p(t):
-    return None if t is None else t.data_ptr()
+    if t is None:
+        return None
+    if (t.dtype is dtype and t.dim() == 2 and t.size(1) == cols and t.size(0) == rows and t.is_contiguous()
+            and t.get_device() == device):
+        return t.data_ptr()
+    raise _Refused
 
 
 def _rows(logits, actions, mask):
-    """The leading arguments of the two calls over rows of logits, and the device; or None."""
+    """The leading arguments of the two calls over rows of logits, and the device."""
     kind = _FLOATS.get(logits.dtype)
-    if kind is None or logits.dim() != 2 or logits.get_device() < 0:
-        return None
-    device = _device()
+    if kind is None or logits.dim() != 2:
+        raise _Refused
     rows, width = logits.shape
     row_stride, stride = logits.stride()
-    if logits.get_device() != device or (stride != 1 and width > 1):
-        return None
+    device = logits.get_device()
+    if device < 0 or (stride != 1 and width > 1) or device != _device():
+        raise _Refused
+    mask_at = None
     mask_stride = action_bytes = 0
     if actions is not None:
         action_bytes = 8 if actions.dtype is torch.int64 else 4
-        if not _vec(actions, rows, device, torch.int64 if action_bytes == 8 else torch.int32):
-            return None
+        actions = _vec(actions, rows, device, torch.int64 if action_bytes == 8 else torch.int32)
     if mask is not None:
-        if mask.dtype not in _BYTES or mask.shape != logits.shape or mask.get_device() != device:
-            return None
+        if (mask.dtype not in _BYTES or mask.dim() != 2 or mask.size(0) != rows or mask.size(1) != width
+                or mask.get_device() != device):
+            raise _Refused
         mask_stride, stride = mask.stride()
         if stride != 1 and width > 1:
-            return None
-    return (logits.data_ptr(), kind, rows, width, row_stride, _p(mask), mask_stride, _p(actions), action_bytes), device
+            raise _Refused
+        mask_at = mask.data_ptr()
+    return logits.data_ptr(), kind, rows, width, row_stride, mask_at, mask_stride, actions, action_bytes, device
 
 
 def logprob(logits, actions=None, logp=None, entropy=None, stats=None, top_ids=None, top_logp=None, mask=None,
@@ -123,24 +133,19 @@ def logprob(logits, actions=None, logp=None, entropy=None, stats=None, top_ids=N
     (rows, 2) with the row's maximum and the log of its sum of exponentials
     above it (what logprob_grad takes), top_ids (rows, k) int32 with top_logp
     (rows, k), k up to 32; float32 where not said otherwise."""
-    a = _rows(logits, actions, mask)
-    if a is None:
+    try:
+        z, kind, rows, width, stride, mask, mask_stride, act, act_bytes, device = _rows(logits, actions, mask)
+        top = 0
+        if top_ids is not None or top_logp is not None:
+            if top_ids is None or top_logp is None or top_ids.dim() != 2:
+                return CUDA_ERROR_INVALID_VALUE
+            top = top_ids.size(1)
+            top_ids, top_logp = _mat(top_ids, rows, top, device, torch.int32), _mat(top_logp, rows, top, device)
+        return lib().b3x_train_logprob_gpu(z, kind, rows, width, stride, mask, mask_stride, act, act_bytes, scale,
+                                           _vec(logp, rows, device), _vec(entropy, rows, device),
+                                           _mat(stats, rows, 2, device), top, top_ids, top_logp, _s(stream, device))
+    except _Refused:
         return CUDA_ERROR_INVALID_VALUE
-    a, device = a
-    rows = a[2]
-    top = 0
-    if top_ids is not None or top_logp is not None:
-        if top_ids is None or top_logp is None or top_ids.dim() != 2:
-            return CUDA_ERROR_INVALID_VALUE
-        top = top_ids.shape[1]
-        if not _mat(top_ids, rows, top, device, torch.int32) or not _mat(top_logp, rows, top, device):
-            return CUDA_ERROR_INVALID_VALUE
-        if top == 0:
-            top_ids = top_logp = None
-    if not (_vec(logp, rows, device) and _vec(entropy, rows, device) and _mat(stats, rows, 2, device)):
-        return CUDA_ERROR_INVALID_VALUE
-    return lib().b3x_train_logprob_gpu(*a, scale, _p(logp), _p(entropy), _p(stats), top, _p(top_ids), _p(top_logp),
-                                       _s(stream, device))
 
 
 def logprob_grad(logits, stats, grad, actions=None, d_logp=None, entropy=None, d_entropy=None, mask=None, scale=1.0,
@@ -149,19 +154,20 @@ def logprob_grad(logits, stats, grad, actions=None, d_logp=None, entropy=None, d
     to the logits, into grad (their shape and type, rows at any stride; the
     logits themselves to overwrite them), from the stats (and entropy, where
     d_entropy is given) that logprob wrote."""
-    a = _rows(logits, actions, mask)
-    if a is None:
+    try:
+        z, kind, rows, width, stride, mask, mask_stride, act, act_bytes, device = _rows(logits, actions, mask)
+        if (grad.dtype is not logits.dtype or grad.dim() != 2 or grad.size(0) != rows or grad.size(1) != width
+                or grad.get_device() != device or stats is None):
+            return CUDA_ERROR_INVALID_VALUE
+        grad_stride, one = grad.stride()
+        if one != 1 and width > 1:
+            return CUDA_ERROR_INVALID_VALUE
+        return lib().b3x_train_logprob_grad_gpu(z, kind, rows, width, stride, mask, mask_stride, act, act_bytes, scale,
+                                                _mat(stats, rows, 2, device), _vec(entropy, rows, device),
+                                                _vec(d_logp, rows, device), _vec(d_entropy, rows, device),
+                                                grad.data_ptr(), grad_stride, _s(stream, device))
+    except _Refused:
         return CUDA_ERROR_INVALID_VALUE
-    a, device = a
-    rows, width = a[2], a[3]
-    if grad.dtype is not logits.dtype or grad.shape != logits.shape or grad.get_device() != device:
-        return CUDA_ERROR_INVALID_VALUE
-    grad_stride, stride = grad.stride()
-    if ((stride != 1 and width > 1) or stats is None or not _mat(stats, rows, 2, device)
-            or not _vec(entropy, rows, device) or not _vec(d_logp, rows, device) or not _vec(d_entropy, rows, device)):
-        return CUDA_ERROR_INVALID_VALUE
-    return lib().b3x_train_logprob_grad_gpu(*a, scale, stats.data_ptr(), _p(entropy), _p(d_logp), _p(d_entropy),
-                                            grad.data_ptr(), grad_stride, _s(stream, device))
 
 
 def advantage(rewards, values, terminals, last_values, advantages, returns=None, gamma=0.99, lam=0.95, lengths=None,
@@ -184,13 +190,16 @@ def advantage(rewards, values, terminals, last_values, advantages, returns=None,
         return CUDA_ERROR_INVALID_VALUE
     if returns is not None and (returns.dtype is not f32 or returns.shape != shape or returns.get_device() != device):
         return CUDA_ERROR_INVALID_VALUE
-    if not _vec(lengths, shape[1], device, torch.int32):
+    try:
+        lengths = _vec(lengths, shape[1], device, torch.int32)
+    except _Refused:
         return CUDA_ERROR_INVALID_VALUE
     strides = _Strides(*rewards.stride(), *values.stride(), *terminals.stride(), *last_values.stride(),
                        *advantages.stride(), *((0, 0) if returns is None else returns.stride()))
     return lib().b3x_train_advantage_gpu(shape[0], shape[1], rewards.data_ptr(), values.data_ptr(), kind,
                                          terminals.data_ptr(), _F32 if terminals.dtype is f32 else _U8,
-                                         last_values.data_ptr(), _p(lengths), advantages.data_ptr(), _p(returns), strides,
+                                         last_values.data_ptr(), lengths, advantages.data_ptr(),
+                                         None if returns is None else returns.data_ptr(), strides,
                                          gamma, lam, _s(stream, device))
 
 
@@ -219,8 +228,9 @@ def grad_norm(grads, max_norm, out, workspace, stream=None):
     sizes = list(map(_numel, grads))
     dtype = grads[0].dtype if grads else torch.float32
     g = _list(grads, sizes, dtype, device) if dtype in _FLOATS else None
-    if (g is None or out is None or not _vec(out, 2, device) or workspace.dtype is not torch.uint8
-            or not workspace.is_contiguous() or workspace.get_device() != device):
+    if (g is None or out.dtype is not torch.float32 or out.shape != (2,) or not out.is_contiguous()
+            or out.get_device() != device or workspace.dtype is not torch.uint8 or not workspace.is_contiguous()
+            or workspace.get_device() != device):
         return CUDA_ERROR_INVALID_VALUE
     counts = array.array("q", sizes)   # named, so that it outlives the call
     return lib().b3x_train_grad_norm_gpu(len(sizes), _addr(g), _FLOATS[dtype], _addr(counts), max_norm,
@@ -271,5 +281,6 @@ def adamw(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2=0.999, 
     counts = array.array("q", sizes)
     return lib().b3x_train_adamw_gpu(n, _addr(p), _FLOATS[pt], _addr(g), _FLOATS[gt], _addr(m), _addr(v), _addr(s),
                                      _E4M3 if f8 else _F32, _addr(c), _addr(counts), _addr(decays), step, lr, beta1,
-                                     beta2, eps, weight_decay, _p(grad_scale), seed is not None,
+                                     beta2, eps, weight_decay,
+                                     None if grad_scale is None else grad_scale.data_ptr(), seed is not None,
                                      (seed or 0) & 0xFFFFFFFF, _s(stream, device))
