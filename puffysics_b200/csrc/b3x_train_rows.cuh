@@ -32,10 +32,15 @@ __device__ __forceinline__ float logit(const Rows& a, long long row, int j) {
 // memory, wherever it starts: vector v holds the elements from v N - head on.
 template <class T> struct Vec { static constexpr int n = 16 / sizeof(T); };
 
+// kAgain: will be read again soon, so it stays in L1.
+template <bool kAgain>
 __device__ __forceinline__ uint4 load16(const void* p) {
     uint4 q;
-    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
+    if (kAgain)
+        asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
+    else
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "l"(p));
     return q;
 }
 
@@ -50,7 +55,7 @@ __device__ __forceinline__ uint32_t nonzero_bytes(uint32_t x) { return ((x & 0x7
 // A row's vectors.  Whole 16 bytes are read wherever they lie within the tensor,
 // so that the ends of a row that starts off a boundary cost no loads of their
 // own: what belongs to its neighbours, or to the space between rows, is replaced.
-template <class T, bool kMask>
+template <class T, bool kMask, bool kAgain = false>
 struct Source {
     static constexpr int N = Vec<T>::n;
     const T* row;
@@ -76,7 +81,7 @@ struct Source {
     // A vector among those.
     __device__ __forceinline__ uint4 inner(int v) const {
         const int j = v * N - head;
-        uint4 q = load16(row + j);
+        uint4 q = load16<kAgain>(row + j);
         if (kMask) keep(q, mask + j);
         return q;
     }
@@ -87,7 +92,7 @@ struct Source {
         const bool ends = j < 0 || j + N > width;
         uint4 q;
         if (!ends || (row + j >= begin && row + j + N <= end)) {
-            q = load16(row + j);
+            q = load16<kAgain>(row + j);
         } else {
             uint32_t* w = &q.x;
             w[0] = w[1] = w[2] = w[3] = 0;

@@ -785,3 +785,19 @@ def test_exports_and_argument_checks_need_no_device(built):
     for args in ((1, ptr, 0, sizes, 0.0, one, one, 1 << 20, n), (1, none, 0, sizes, 1.0, one, one, 1 << 20, n), (1, ptr, 0, sizes, 1.0, n, one, 1 << 20, n),
                  (1, ptr, 0, sizes, 1.0, one, one, 8, n), (1, ptr, 3, sizes, 1.0, one, one, 1 << 20, n), (1, ptr, 0, neg, 1.0, one, one, 1 << 20, n)):
         assert L.b3x_train_grad_norm_gpu(*args) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eight_bit", [False, True])
+def test_hover_training_learns(eight_bit):
+    """The example's loop: a policy that began at random holds its height far better after 40 iterations (a step's
+    reward is at most 1, and 0 at two metres' error)."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "hover_train.py")
+    spec = importlib.util.spec_from_file_location("hover_train", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    got = module.run(envs=1024, iterations=40, eight_bit=eight_bit)
+    assert all(math.isfinite(x) for x in got)
+    assert sum(got[-4:]) / 4 > sum(got[1:8]) / 7 + 0.3, got
