@@ -17,6 +17,7 @@ actions that are none, terminals and lengths.
 """
 import array
 import ctypes
+import operator
 import os
 
 import torch
@@ -36,6 +37,7 @@ _BYTES = {torch.uint8: _U8, torch.bool: _U8}
 _Strides = ctypes.c_longlong * 11
 _numel, _dense, _where, _pointer = (torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.get_device,
                                     torch.Tensor.data_ptr)
+_kind = operator.attrgetter("dtype")
 
 _lib = None
 
@@ -206,8 +208,8 @@ def advantage(rewards, values, terminals, last_values, advantages, returns=None,
 def _list(tensors, sizes, dtype, device):
     """Pointers of a list of dense tensors on the device, of one type and these
     element counts; None where they are not."""
-    if (list(map(_numel, tensors)) != sizes or not all(map(_dense, tensors)) or any(t.dtype is not dtype for t in tensors)
-            or any(map(device.__ne__, map(_where, tensors)))):
+    if (list(map(_numel, tensors)) != sizes or not all(map(_dense, tensors)) or {dtype} != {dtype, *map(_kind, tensors)}
+            or {device} != {device, *map(_where, tensors)}):
         return None
     return array.array("Q", map(_pointer, tensors))
 
