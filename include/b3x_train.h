@@ -98,7 +98,8 @@ B3X_TRAIN_API int b3x_train_logprob_grad_gpu(const void* logits, int type, long 
  * type B3X_F32, B3X_BF16 or B3X_F16, terminals B3X_F32 or B3X_U8; the rest is
  * B3X_F32.  returns may be NULL.  strides, in elements, per step and per
  * environment: rewards, values, terminals (2 each), last_values (1),
- * advantages, returns (2 each).  Outputs overlap nothing. */
+ * advantages, returns (2 each).  Outputs overlap nothing.  steps and envs are at
+ * most 2^30 each. */
 B3X_TRAIN_API int b3x_train_advantage_gpu(long long steps, long long envs, const float* rewards,
         const void* values, int value_type, const void* terminals, int terminal_type, const void* last_values,
         const int* lengths, float* advantages, float* returns, const long long strides[11], float gamma,
@@ -128,7 +129,8 @@ B3X_TRAIN_API int b3x_train_grad_norm_gpu(int count, const void* const* grads, i
  * m and sqrt(v) as e4m3, and scales[k] two floats for each B3X_TRAIN_BLOCK
  * elements, 448 of a code standing for the block's largest: value = code *
  * scale.  A block whose largest is under 2^-100 is held as zeros; sqrt(v) above
- * zero never rounds to zero.
+ * zero never rounds to zero.  A NaN or infinity makes its whole block's
+ * moments NaN (with moments in 32 bits its own alone).
  *
  * copies (NULL: none, or NULL entries): bf16 tensors that get the new
  * parameters, rounded to nearest.  decays (NULL: weight_decay for all): a

@@ -157,6 +157,13 @@ __device__ __forceinline__ float warp_most(float x) {
 // so that every load and store is a whole line however wide its type.  The
 // moments' operations round one by one: their codes are those of the plain
 // formula, bit for bit.
+//
+// 168 M parameters.  In 32 bits throughout 704 us, 6.8 TB/s, a little over the
+// copy rate: bound by memory (bf16 parameters and gradients 558 us, 6.8 TB/s).
+// With 8-bit moments, bf16 parameters and gradients and stochastic rounding 460
+// us, 58% of the copy rate: bound by issued instructions, 81 an element (issue
+// slots 78% busy, the integer pipe 64%), of which the two hashes are 19 and the
+// codes 12.
 template <class P, class G, bool kF8, bool kRandom, bool kWhole>
 __device__ __forceinline__ void update(const Tensor& t, const Hyper& h, const float gs, const long long base, const int lane) {
     const long long n = t.n;

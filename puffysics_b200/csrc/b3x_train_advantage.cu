@@ -177,7 +177,8 @@ __device__ __forceinline__ Pair scan_lanes(Pair p, int apart, int width) {
 }
 
 // Many environments, time consecutive in memory: `group` lanes an environment,
-// 4 steps a lane, from the last steps to the first.
+// 4 steps a lane, from the last steps to the first: 64 steps of 65,536
+// environments 17 us, 256 of 16,384 17 us (the bytes alone 13).
 constexpr int kRowThreads = 256;
 
 template <class V, class D>
@@ -231,6 +232,13 @@ struct Shared {
 // several turns of the block, from the last steps to the first, each with what
 // the one before carried; the blocks of a cluster go through their part once
 // before, for its pair alone (their second reading comes from L2).
+//
+// 64 steps of 4,096 environments side by side: 2.8 us, latency.  256 steps of
+// 16,384: 18 us (4.7 TB/s, 73% of the copy rate).  1,024 environments of up to
+// 8,191 steps one after the other, bf16 values: 34 us (69%), bound by the turns'
+// chains of loads and joins at 64 registers a thread; loading a turn ahead took
+// registers and 46 us (at 4 steps a thread, where this took 39).  65,536 steps
+// of one environment: 13 us on a cluster's eight SMs.
 template <class V, class D, bool kVec>
 __global__ void __launch_bounds__(kMaxThreads) advantage_kernel(const Rollout a, int env_bits, int cluster) {
     constexpr int kSteps = kBlockSteps;
