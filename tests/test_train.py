@@ -801,3 +801,146 @@ def test_hover_training_learns(eight_bit):
     got = module.run(envs=1024, iterations=40, eight_bit=eight_bit)
     assert all(math.isfinite(x) for x in got)
     assert sum(got[-4:]) / 4 > sum(got[1:8]) / 7 + 0.3, got
+
+
+# ---- more rows, longer lists, larger offsets -------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("rows,width,pad,dtype,top", [
+    (1300, 700, 1, "f32", 20), (1300, 2500, 0, "bf16", 32), (1200, 5001, 2, "f16", 5), (1200, 1100, 0, "bf16", 0),
+    (700, 3000, 0, "bf16", 20), (700, 1500, 3, "f32", 1)])
+def test_logprob_more_rows_than_blocks(rows, width, pad, dtype, top, masked):
+    store = make_logits(rows, width, pad, dtype, width)
+    rng = np.random.default_rng(rows)
+    mask = torch.from_numpy((rng.random((rows, width)) < 0.6).astype(np.uint8)) if masked else None
+    check_logprob(store, width, torch.from_numpy(rng.integers(0, width, rows)), mask, 1.3, top)
+
+
+@pytest.mark.gpu
+def test_logprob_offsets_beyond_32_bits():
+    """Rows 1.5e9 elements apart: the last one begins beyond 2^31 elements."""
+    stride, width = 1500000000, 1003
+    store = torch.empty(2 * stride + width, dtype=torch.bfloat16, device="cuda")
+    z = torch.as_strided(store, (3, width), (stride, 1))
+    z.copy_(torch.from_numpy(np.random.default_rng(0).normal(0, 2, (3, width))))
+    out, ref = outputs(3, 20), outputs(3, 20)
+    act = torch.tensor([0, 5, 1002], device="cuda")
+    dense = z.contiguous()
+    for a, o in ((z, out), (dense, ref)):
+        assert train.logprob(a, act, **o) == 0
+    for k in out:
+        if k in ("top_ids",):
+            assert torch.equal(out[k], ref[k])
+        else:
+            assert (out[k] - ref[k]).abs().max() <= 64 * E * (1 + ref[k].abs().max())
+    ones = torch.ones(3, device="cuda")
+    want = torch.empty_like(dense)
+    assert train.logprob_grad(dense, out["stats"], want, actions=act, d_logp=ones, entropy=out["entropy"], d_entropy=ones) == 0
+    assert train.logprob_grad(z, out["stats"], z, actions=act, d_logp=ones, entropy=out["entropy"], d_entropy=ones) == 0
+    assert torch.equal(z, want)
+
+
+def advantage_many(r, v, d, last, gamma, lam):
+    """advantage_oracle for all environments at once, all of full length."""
+    T, N = r.shape
+    adv, tol = np.zeros((T, N)), np.zeros((T, N))
+    ahead, after, s, k = np.zeros(N), last, np.zeros(N), np.zeros(N)
+    for t in range(T - 1, -1, -1):
+        on = d[t] == 0
+        a = np.where(on, gamma * lam, 0.0)
+        ahead = r[t] + np.where(on, gamma * after, 0.0) - v[t] + a * ahead
+        k = a * (k + s)
+        s = np.abs(r[t]) + np.where(on, np.abs(gamma * after), 0.0) + np.abs(v[t]) + a * s
+        adv[t], tol[t], after = ahead, 2 * E * (k + 8 * s), v[t]
+    return adv, tol
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["time", "env"])
+@pytest.mark.parametrize("steps,envs", [(64, 4096), (300, 5000), (127, 20001), (3, 70000), (2000, 700)])
+def test_advantage_of_many_environments(steps, envs, order):
+    rng = np.random.default_rng(steps)
+    r, v = (rng.normal(0, 1, (steps, envs)).astype(np.float32) for _ in range(2))
+    d = (rng.random((steps, envs)) < 0.02).astype(np.float32)
+    last = rng.normal(0, 1, envs).astype(np.float32)
+
+    def lay(x):
+        x = torch.from_numpy(x).cuda()
+        return x if order == "time" else x.t().contiguous().t()
+    adv, ret = lay(np.zeros_like(r)), lay(np.zeros_like(r))
+    assert train.advantage(lay(r), lay(v), lay(d), torch.from_numpy(last).cuda(), adv, ret, gamma=0.99, lam=0.95) == 0
+    g32 = float(np.float32(0.99))
+    a32 = float(np.float32(np.float32(0.99) * np.float32(0.95)))
+    want, tol = advantage_many(*(x.astype(np.float64) for x in (r, v, d, last)), g32, a32 / g32)
+    near(adv.cpu().numpy(), want, tol)
+    near(ret.cpu().numpy(), want + v, tol + E * np.abs(want + v))
+
+
+@pytest.mark.gpu
+def test_advantage_offsets_beyond_32_bits():
+    """Steps 1.1e9 elements apart."""
+    stride = 1100000000
+    store = torch.empty(2 * stride + 8, device="cuda")
+    r = torch.as_strided(store, (3, 5), (stride, 1))
+    r.copy_(torch.arange(15.0).view(3, 5))
+    dense = r.contiguous()
+    v, d, last = torch.ones((3, 5), device="cuda"), torch.zeros((3, 5), device="cuda"), torch.zeros(5, device="cuda")
+    got, want = torch.empty((3, 5), device="cuda"), torch.empty((3, 5), device="cuda")
+    assert train.advantage(r, v, d, last, got) == 0 and train.advantage(dense, v, d, last, want) == 0
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("state", ["f32", "f8"])
+def test_adamw_of_millions(state):
+    """Chunks of several turns: the same bits as the plain formula where it is held in 8 bits, in 32 for m and v."""
+    sizes = [10000001, 37, 300000]
+    s = make_adam(sizes, "f32", "f32", state, 3)
+    before = {k: None if v is None else [host(t).copy() for t in v] for k, v in s.items() if k != "whole"}
+    ws, norm = torch.empty(train.grad_norm_workspace_bytes(), dtype=torch.uint8, device="cuda"), torch.empty(2, device="cuda")
+    assert train.grad_norm(s["grads"], INF, norm, ws) == 0
+    want = math.sqrt(sum(float((g.double() ** 2).sum()) for g in s["grads"]))
+    assert abs(float(norm[0]) - want) <= 2 * E * want and float(norm[1]) == 1.0
+    assert train.adamw(s["params"], s["grads"], s["m"], s["v"], 3, weight_decay=0.0, scales=s["scales"], seed=7, **H) == 0
+    b1, c1, b2, c2 = (np.float32(x) for x in (0.9, 1 - 0.9, 0.95, 1 - 0.95))
+    for k, n in enumerate(sizes):
+        g = before["grads"][k]
+        if state == "f32":
+            m, v = before["m"][k], before["v"][k]
+        else:
+            sc = before["scales"][k].repeat(256, 0)[:n]
+            m, r = np_decode(before["m"][k]) * sc[:, 0], np_decode(before["v"][k]) * sc[:, 1]
+            v = r * r
+        m, v = m * b1 + g * c1, v * b2 + (g * g) * c2
+        if state == "f32":
+            assert np.array_equal(host(s["m"][k]), m) and np.array_equal(host(s["v"][k]), v)
+        else:
+            bits = np_hash(n, k, 3, 7)
+            root = np.sqrt(v)
+            cm, sm = np_pack(m, bits & np.uint64(0xFFFF))
+            cv, sv = np_pack(root, bits >> np.uint64(16))
+            cv = np.where((cv == 0) & (root > 0) & (sv.repeat(256)[:n] > 0), 1, cv)
+            assert np.array_equal(host(s["scales"][k]), np.stack((sm, sv), 1))
+            assert np.array_equal(host(s["m"][k]), cm) and np.array_equal(host(s["v"][k]), cv)
+
+
+@pytest.mark.gpu
+def test_adamw_elements_beyond_32_bits():
+    """A tensor of 2^32 + 700 elements (34 GB with its gradient and moments): the last ones as any others."""
+    n, tail = (1 << 32) + 700, 1000
+    p, g = (torch.zeros(n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    m, v = (torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+    sc = torch.zeros(((n + 255) // 256, 2), device="cuda")
+    first = (n - tail) // 256 * 256
+    grads = (np.random.default_rng(0).normal(0, 1, n - first)).astype(np.float32)
+    g[first:] = torch.from_numpy(grads).cuda()
+    grads = host(g[first:])
+    assert train.adamw([p], [g], [m], [v], 1, 1e-2, scales=[sc], weight_decay=0.0, seed=11) == 0
+    M = np.uint64(0xFFFFFFFF)
+    i = np.arange(first, n, dtype=np.uint64)
+    key = np_mix(np.array([(11 + 0x6A09E667) & 0xFFFFFFFF], np.uint64))[0]
+    bits = np_mix(((i & M) * np.uint64(0x9E3779B1) + (i >> np.uint64(32)) * np.uint64(0x6A09E667) + key) & M)
+    mm = grads * np.float32(1 - 0.9)
+    cm, sm = np_pack(mm, bits & np.uint64(0xFFFF))
+    assert np.array_equal(host(m[first:]), cm) and np.array_equal(host(sc[first // 256:, 0]), sm)
+    assert (p[:1000] == 0).all() and (p[first:] != 0).any()
