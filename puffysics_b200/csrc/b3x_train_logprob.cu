@@ -235,6 +235,31 @@ __device__ __forceinline__ uint32_t merge_lanes(uint32_t key, uint32_t mirrored)
     return key;
 }
 
+// Of a warp's 32 vectors from v on (those before v1) the logits with this key, in
+// order, as entries from out[got] on, no more than `need` in all; how many there are then.
+template <class T, class S>
+__device__ __forceinline__ int take_equal(const S& src, int v, int v1, uint32_t key, uint64_t* out, int need, int got) {
+    constexpr int N = Vec<T>::n;
+    v += threadIdx.x % 32;
+    const uint4 q = v < v1 ? src.load(v) : no_vector<T>();
+    uint32_t bits = 0;
+#pragma unroll
+    for (int n = 0; n < N; n++) bits |= key_of(element<T>(q, n)) == key ? 1u << n : 0;
+    int at = __popc(bits);
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const int before = __shfl_up_sync(~0u, at, o);
+        if (threadIdx.x % 32 >= o) at += before;
+    }
+    const int all = __shfl_sync(~0u, at, 31);
+    at += got - __popc(bits);
+    while (bits && at < need) {
+        out[at++] = entry_of(key, v * N - src.head + __ffs(bits) - 1);
+        bits &= bits - 1;
+    }
+    return min(need, got + all);
+}
+
 // The sums of a row of logits of 1e38, whose products with c are beyond the
 // floats: x = c (z - m).  `by`: threads that share the row.
 template <class T, bool kMask>
@@ -303,7 +328,7 @@ template <> __device__ __forceinline__ float lowest<__half>() { return -65504.0f
 
 template <class T, bool kMask, bool kTop, int L, bool kWalk>
 __global__ void __launch_bounds__(kRowThreads, kTop ? 4 : 5) lanes_kernel(Rows a, Out o) {
-    constexpr int N = Vec<T>::n, U = 4, kRows = 32 / L, kCap = kRowFound / kRows;
+    constexpr int N = Vec<T>::n, U = 4, kRows = 32 / L, kCap = kRowFound / kRows, kFew = L == 32 ? 96 : kCap;
     __shared__ uint64_t entries[kTop ? kRowThreads / L : 1][kTop ? kCap : 1];
     __shared__ __align__(16) uint32_t best[kTop && L < 32 ? kRowThreads / L : 1][kTop && L < 32 ? U * L : 1];
     __shared__ int found[kTop ? kRowThreads / L : 1];
@@ -421,13 +446,34 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 4 : 5) lanes_kernel(Rows a
         }
     }
     __syncwarp();
-    const int n = found[here];
-    const bool ranked = n <= kCap && p.m == p.m;
+    int n = found[here];
+    bool ranked = n <= kFew && p.m == p.m;
     if (ranked) {
         for (int i = lane; i < n; i += L) {
             const int j = (int)entries[here][i];
             entries[here][i] = entry_of(key_of(to_float(src.row[j])), j);
         }
+    } else if (L == 32 && p.m == p.m) {
+        // many logits, by far the most equal to the threshold: all above it, then the first of those
+        const uint32_t key = key_of(z);
+        __syncwarp();
+        if (lane == 0) found[here] = 0;
+        __syncwarp();
+        for (int v = lane; v < nv; v += 32) {
+            const uint4 x = src.load(v);
+            if (key_of(most<T>(x)) <= key) continue;
+            for (int i = 0; i < N; i++) {
+                const uint32_t k = key_of(element<T>(x, i));
+                if (k <= key) continue;
+                const int at = atomicAdd(&found[here], 1);
+                if (at >= kCap) break;
+                entries[here][at] = entry_of(k, v * N - src.head + i);
+            }
+        }
+        __syncwarp();
+        n = found[here];
+        for (int v = 0; v < nv && n < o.top; v += 32) n = take_equal<T>(src, v, nv, key, entries[here], o.top, n);
+        ranked = n <= kCap;
     }
     __syncwarp();
     if (ranked && on) {
@@ -440,7 +486,7 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 4 : 5) lanes_kernel(Rows a
         for (int i = n + lane; i < o.top; i += L) write_top(o, row, i, 0, r, a.scale);
     }
     if (__all_sync(~0u, ranked)) return;
-    // many equal logits, or NaN: each time the best one after the last
+    // too many logits to rank, or NaN: each time the best one after the last
     uint64_t last = ~0ull;
     for (int k = 0; k < o.top; k++) {
         uint64_t top = 0;
@@ -465,7 +511,7 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 4 : 5) lanes_kernel(Rows a
 constexpr int kUnroll = 4;           // vectors a thread has in flight
 constexpr int kTile = 32 * kUnroll;  // vectors a warp takes at a time
 constexpr int kGroups = 512;         // groups of consecutive vectors whose maxima are kept
-constexpr int kFound = 512;          // logits at or above the threshold that are ranked at once
+constexpr int kFound = 256;          // logits at or above the threshold that are ranked at once
 constexpr int kMaxWarps = 16;
 constexpr int kMaxCluster = 8;
 constexpr int kSmallWarps = 4, kSmallBlocks = 8;   // of a block where there are many rows
@@ -501,7 +547,8 @@ __device__ __forceinline__ uint32_t remote(const void* p, uint32_t rank) {
 __device__ __forceinline__ float remote_float(const void* p, uint32_t rank) { return __uint_as_float(remote(p, rank)); }
 
 // The K largest entries among the vectors of some groups (or all): each time
-// the best one after the last.  Only for rows with many equal logits or NaN.
+// the best one after the last.  Only for rows with NaN, or with more logits above
+// the threshold than are ranked at once.
 template <class T, bool kMask>
 __device__ __noinline__ void search(const Source<T, kMask>& src, Shared& sh, int v0, int v1, int shift, const int* order,
                                     int groups, int top) {
@@ -552,7 +599,8 @@ __device__ __forceinline__ void gather(const Source<T, kMask>& src, Shared& sh, 
         const uint32_t key = key_of(element<T>(q, n));
         if (key < threshold) continue;
         const int at = atomicAdd(&sh.found, 1);
-        if (at < kFound) sh.entries[at] = entry_of(key, v * Vec<T>::n - src.head + n);
+        if (at >= kFound) return;   // too many to rank already
+        sh.entries[at] = entry_of(key, v * Vec<T>::n - src.head + n);
     }
 }
 
@@ -666,28 +714,49 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallB
         if (p.m != p.m) {
             search<T, kMask>(src, sh, v0, v1, shift, nullptr, groups, o.top);
         } else {
-            if (kOnce) {
-#pragma unroll
-                for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v0 + warp * kTile + u * 32 + lane, threshold);
-            } else {
+            if (!kOnce) {
                 for (int g = threadIdx.x; g < groups; g += blockDim.x)
                     if (sh.group[g] >= threshold) sh.order[atomicAdd(&sh.chosen, 1)] = g;
                 __syncthreads();
+            }
+            const auto collect = [&](uint32_t least) {
+                if (kOnce) {
+#pragma unroll
+                    for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v0 + warp * kTile + u * 32 + lane, least);
+                    return;
+                }
                 const int again = sh.chosen << shift;
-                for (int i = threadIdx.x; i < again; i += blockDim.x * kUnroll) {
+                for (int i = threadIdx.x; i < again && *(volatile int*)&sh.found <= kFound; i += blockDim.x * kUnroll) {
                     int v[kUnroll];
+                    uint4 w[kUnroll];
 #pragma unroll
                     for (int u = 0; u < kUnroll; u++) {
-                        const int k = i + u * blockDim.x;
-                        v[u] = k < again ? v0 + (sh.order[k >> shift] << shift) + (k & ((1 << shift) - 1)) : v1;
-                        if (v[u] >= 2 && v[u] < min(v1, src.last())) q[u] = src.inner(v[u]);
-                        else q[u] = v[u] < v1 ? src.load(v[u]) : no_vector<T>();
+                        const int k = i + u * blockDim.x, g = k < again ? sh.order[k >> shift] : -1;
+                        v[u] = g >= 0 && sh.group[g] >= least ? v0 + (g << shift) + (k & ((1 << shift) - 1)) : v1;
+                        if (v[u] >= 2 && v[u] < min(v1, src.last())) w[u] = src.inner(v[u]);
+                        else w[u] = v[u] < v1 ? src.load(v[u]) : no_vector<T>();
                     }
 #pragma unroll
-                    for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v[u], threshold);
+                    for (int u = 0; u < kUnroll; u++) gather(src, sh, w[u], v[u], least);
                 }
-            }
+            };
+            collect(threshold);
             __syncthreads();
+            if (sh.found > kFound) {   // many logits equal to the threshold: all above it, then the first of those
+                __syncthreads();
+                if (threadIdx.x == 0) sh.found = 0;
+                __syncthreads();
+                collect(threshold + 1);
+                __syncthreads();
+                if (warp == 0 && sh.found < o.top) {
+                    int n = sh.found;
+                    for (int v = v0; v < v1 && n < o.top; v += 32)
+                        if (kOnce || shift != 5 || sh.group[(v - v0) >> 5] >= threshold)
+                            n = take_equal<T>(src, v, v1, threshold, sh.entries, o.top, n);
+                    if (lane == 0) sh.found = n;
+                }
+                __syncthreads();
+            }
             const int found = sh.found;
             if (found <= kFound) {
                 rank_entries(sh.entries, found, o.top, sh.list);
