@@ -615,6 +615,35 @@ __device__ __noinline__ void best_groups(Shared& sh, int groups, int top) {
     __syncthreads();
 }
 
+// The alternatives of a row with more logits at the threshold than are ranked at
+// once, by far the most equal to it: all above it, then the first of those.
+template <class T, bool kMask, bool kOnce>
+__device__ __noinline__ void crowded(const Source<T, kMask>& src, Shared& sh, int v0, int v1, int shift, int groups, int top,
+                                     uint32_t threshold) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.found = 0;
+    __syncthreads();
+    for (int v = v0 + threadIdx.x; v < v1; v += blockDim.x)
+        if (kOnce || sh.group[(v - v0) >> shift] > threshold) gather(src, sh, src.load(v), v, threshold + 1);
+    __syncthreads();
+    if (threadIdx.x < 32 && sh.found < top) {
+        int n = sh.found;
+        for (int v = v0; v < v1 && n < top; v += 32)
+            if (kOnce || sh.group[(v - v0) >> shift] >= threshold) n = take_equal<T>(src, v, v1, threshold, sh.entries, top, n);
+        if (threadIdx.x == 0) sh.found = n;
+    }
+    __syncthreads();
+    const int found = sh.found;
+    if (found <= kFound) {
+        rank_entries(sh.entries, found, top, sh.list);
+    } else if (kOnce) {
+        search<T, kMask>(src, sh, v0, v1, 0, nullptr, v1 - v0, top);
+    } else {
+        best_groups(sh, groups, top);
+        search<T, kMask>(src, sh, v0, v1, shift, sh.order, min(top, groups), top);
+    }
+}
+
 // One block, or one cluster of blocks, a row; the row is read once.  kOnce: each
 // warp has one tile, which stays in its registers.  Otherwise the warps walk
 // over the row with their sums running.
@@ -719,53 +748,28 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallB
                     if (sh.group[g] >= threshold) sh.order[atomicAdd(&sh.chosen, 1)] = g;
                 __syncthreads();
             }
-            const auto collect = [&](uint32_t least) {
-                if (kOnce) {
+            if (kOnce) {
 #pragma unroll
-                    for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v0 + warp * kTile + u * 32 + lane, least);
-                    return;
-                }
+                for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v0 + warp * kTile + u * 32 + lane, threshold);
+            } else {
                 const int again = sh.chosen << shift;
                 for (int i = threadIdx.x; i < again && *(volatile int*)&sh.found <= kFound; i += blockDim.x * kUnroll) {
                     int v[kUnroll];
-                    uint4 w[kUnroll];
 #pragma unroll
                     for (int u = 0; u < kUnroll; u++) {
-                        const int k = i + u * blockDim.x, g = k < again ? sh.order[k >> shift] : -1;
-                        v[u] = g >= 0 && sh.group[g] >= least ? v0 + (g << shift) + (k & ((1 << shift) - 1)) : v1;
-                        if (v[u] >= 2 && v[u] < min(v1, src.last())) w[u] = src.inner(v[u]);
-                        else w[u] = v[u] < v1 ? src.load(v[u]) : no_vector<T>();
+                        const int k = i + u * blockDim.x;
+                        v[u] = k < again ? v0 + (sh.order[k >> shift] << shift) + (k & ((1 << shift) - 1)) : v1;
+                        if (v[u] >= 2 && v[u] < min(v1, src.last())) q[u] = src.inner(v[u]);
+                        else q[u] = v[u] < v1 ? src.load(v[u]) : no_vector<T>();
                     }
 #pragma unroll
-                    for (int u = 0; u < kUnroll; u++) gather(src, sh, w[u], v[u], least);
+                    for (int u = 0; u < kUnroll; u++) gather(src, sh, q[u], v[u], threshold);
                 }
-            };
-            collect(threshold);
+            }
             __syncthreads();
-            if (sh.found > kFound) {   // many logits equal to the threshold: all above it, then the first of those
-                __syncthreads();
-                if (threadIdx.x == 0) sh.found = 0;
-                __syncthreads();
-                collect(threshold + 1);
-                __syncthreads();
-                if (warp == 0 && sh.found < o.top) {
-                    int n = sh.found;
-                    for (int v = v0; v < v1 && n < o.top; v += 32)
-                        if (kOnce || shift != 5 || sh.group[(v - v0) >> 5] >= threshold)
-                            n = take_equal<T>(src, v, v1, threshold, sh.entries, o.top, n);
-                    if (lane == 0) sh.found = n;
-                }
-                __syncthreads();
-            }
             const int found = sh.found;
-            if (found <= kFound) {
-                rank_entries(sh.entries, found, o.top, sh.list);
-            } else if (kOnce) {
-                search<T, kMask>(src, sh, v0, v1, 0, nullptr, v1 - v0, o.top);
-            } else {
-                best_groups(sh, groups, o.top);
-                search<T, kMask>(src, sh, v0, v1, shift, sh.order, min(o.top, groups), o.top);
-            }
+            if (found <= kFound) rank_entries(sh.entries, found, o.top, sh.list);
+            else crowded<T, kMask, kOnce>(src, sh, v0, v1, shift, groups, o.top, threshold);
         }
         __syncthreads();
     }
