@@ -816,9 +816,10 @@ static_assert(kMaxCluster * B3X_TRAIN_MAX_TOP <= kFound, "the blocks' alternativ
 
 template <class T, bool kMask, bool kTop>
 int launch_long(const Rows& a, const Out& o, int nv, cudaStream_t s) {
-    // a cluster a row while rows alone leave SMs idle and each block keeps 512 vectors
+    // A cluster a row while rows alone leave SMs idle and each block keeps 1,024 vectors: 8 rows of 131,072 bf16 with 20
+    // alternatives 9.8 us, by single blocks 13.5; 8 rows of 32,768 8.1 us so, by two blocks each 10.2.
     int cluster = 1;
-    while (cluster < kMaxCluster && a.rows * cluster * 2 <= 296 && nv / (cluster * 2) >= 512) cluster *= 2;
+    while (cluster < kMaxCluster && a.rows * cluster * 2 <= 296 && nv / (cluster * 2) >= 1024) cluster *= 2;
     int each = (nv + cluster - 1) / cluster;
     // Rows for every SM several times over: small blocks, whose ends overlap (4,096 rows of 131,072 bf16 with 20
     // alternatives 254 us with 16 warps, 221 with 4; 2,048 masked rows of 50,001 120 us with 16, 75 with 2).  Fewer:
