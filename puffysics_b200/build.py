@@ -7,9 +7,11 @@ contraction), -prec-div=true / -prec-sqrt=true / -ftz=false (IEEE division,
 square root and denormals).  With them every float expression of the step
 rounds exactly like the reference's CPU build with -ffp-contract=off.
 """
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -43,6 +45,9 @@ TRAIN_SRC = [os.path.join(PKG, "csrc", "b3x_train_%s.cu" % n) for n in ("logprob
 TRAIN_LIB = os.path.join(LIB_DIR, "libb3train.so")
 TRAIN_HEADERS = [os.path.join(ROOT, "include", "b3x_train.h"), os.path.join(PKG, "csrc", "b3x_train_common.cuh"),
                  os.path.join(PKG, "csrc", "b3x_train_rows.cuh")]
+# their Python side, compiled against torch's headers (b3train_py.so)
+TRAIN_PY_SRC = os.path.join(PKG, "csrc", "b3x_train_py.cpp")
+TRAIN_PY_LIB = os.path.join(LIB_DIR, "b3train_py.so")
 # capacity configurations the host scene builders are compiled for:
 # name -> (bodies, shapes, contacts, joints)
 SCENE_CONFIGS = {"hover": (2, 2, 4, 1), "stack": (9, 9, 32, 1), "chain": (12, 12, 32, 10),
@@ -69,6 +74,7 @@ THREAD_MODES = {"stackil": ["-DB3_INTERLEAVE_CONTACTS"], "chainil": ["-DB3_INTER
                 "hoveruf": ["-include", os.path.join(PKG, "scenes", "b3_test_forces.h")],
                 "chainart": ["-DB3_ART_CONTACTS=1"]}
 CC = os.environ.get("CC", "gcc")
+CXX = os.environ.get("CXX", "g++")
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc" if os.path.exists("/usr/local/cuda/bin/nvcc") else "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -117,6 +123,27 @@ def train_cmd(extra=()):
             + list(extra) + TRAIN_SRC + ["-o", TRAIN_LIB])
 
 
+def train_py_cmd():
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"]]
+    libs = os.path.join(torch, "lib")
+    return ([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
+            + [x for d in include for x in ("-isystem", d)] + ["-I" + os.path.join(ROOT, "include"), TRAIN_PY_SRC,
+               "-L" + LIB_DIR, "-lb3train", "-L" + libs, "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10",
+               "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + libs, "-o", TRAIN_PY_LIB])
+
+
+def build_train_py(force=False):
+    """The training operators' Python side (after libb3train.so, which it links)."""
+    if not force and not _newer(TRAIN_PY_LIB, [TRAIN_PY_SRC, TRAIN_HEADERS[0], __file__]):
+        return
+    cmd = train_py_cmd()
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("training operators' Python side failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+
+
 def build_thread_libs(force=False):
     """The per-thread step launchers, one per capacity configuration, the
     hover environment library and the training operators, compiled
@@ -156,7 +183,8 @@ def up_to_date():
     return (not _newer(LIB, deps) and not any(_newer(scenes_lib(n), [SCENES_SRC] + HEADERS) for n in SCENE_CONFIGS)
             and not any(_newer(thread_lib(n), thread_deps) for n in thread_lib_names())
             and not _newer(HOVER_LIB, [HOVER_SRC, __file__] + THREAD_DEPS + HOVER_HEADERS)
-            and not _newer(TRAIN_LIB, TRAIN_SRC + TRAIN_HEADERS + [__file__]))
+            and not _newer(TRAIN_LIB, TRAIN_SRC + TRAIN_HEADERS + [__file__])
+            and not _newer(TRAIN_PY_LIB, [TRAIN_PY_SRC, TRAIN_HEADERS[0], __file__]))
 
 
 def build_scenes(force=False):
@@ -183,6 +211,7 @@ def build(force=False, verbose=False):
     os.makedirs(LIB_DIR, exist_ok=True)
     build_scenes(force)
     build_thread_libs(force)
+    build_train_py(force)
     if not force and not _newer(LIB, SOURCES + HEADERS + [__file__]):
         return LIB
     cmd = nvcc_cmd(extra=["-Xptxas", "-v"] if verbose else [])
