@@ -160,8 +160,8 @@ __device__ __forceinline__ float warp_most(float x) {
 //
 // 168 M parameters.  In 32 bits throughout 704 us, 6.8 TB/s, a little over the
 // copy rate: bound by memory (bf16 parameters and gradients 558 us, 6.8 TB/s).
-// With 8-bit moments, bf16 parameters and gradients and stochastic rounding 460
-// us, 58% of the copy rate: bound by issued instructions, 81 an element (issue
+// With 8-bit moments, bf16 parameters and gradients and stochastic rounding 449
+// us, 60% of the copy rate: bound by issued instructions, 81 an element (issue
 // slots 78% busy, the integer pipe 64%), of which the two hashes are 19 and the
 // codes 12.
 template <class P, class G, bool kF8, bool kRandom, bool kWhole>

@@ -655,11 +655,11 @@ __device__ __noinline__ void crowded(const Source<T, kMask>& src, Shared& sh, in
 // from L2.
 //
 // 4,096 rows of 131,072 bf16: 177 us without alternatives (6.1 TB/s, 94% of the
-// copy rate), 213 with 20 (78%).  An exponential a logit keeps the special
+// copy rate), 219 with 20 (76%).  An exponential a logit keeps the special
 // function unit half busy; the rest of the time is the loads' latency at 64
 // registers a thread, and each row's end (sorting, ranking), which other blocks
 // of the SM cover in part.  12 blocks an SM instead of 8 spill (267 us).  8 rows,
-// a cluster of 8 blocks each: 4.8 us without alternatives, 9.3 with 20, all of it
+// a cluster of 8 blocks each: 4.6 us without alternatives, 9.8 with 20, all of it
 // latency.
 template <class T, bool kMask, bool kTop, bool kOnce, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallBlocks) long_kernel(Rows a, Out o, int cluster, int shift) {

@@ -28,7 +28,7 @@ constexpr int kMaxCluster = 8;
 // 2^bits threads a row (a cluster's blocks together where it has more than one),
 // 16 bytes of logits and of gradients at a time; bound by memory (2,048 rows of
 // 65,536 bf16: 92 us, 5.8 TB/s, 91% of the copy rate; 4,096 rows of 50,001: 156
-// us, 82%; masked 61%, by the mask's instructions).  With
+// us, 81%; masked 61%, by the mask's instructions).  With
 // e = log p_j the gradient is p_j (B e + A) with A = -scale (g + h H) and
 // B = -scale h, and scale g more at the action.
 template <class T, bool kMask>
