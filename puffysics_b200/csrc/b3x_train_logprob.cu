@@ -524,6 +524,7 @@ struct Shared {
     int order[kGroups];
     int chosen, found;
     uint64_t list[B3X_TRAIN_MAX_TOP]; // this block's alternatives
+    uint64_t joined[B3X_TRAIN_MAX_TOP];
     uint64_t entries[kFound];
     uint64_t warp_best[kMaxWarps];
     float2 far[kMaxWarps];
@@ -584,6 +585,7 @@ __device__ __forceinline__ void rank_entries(const uint64_t* entries, int n, int
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const uint64_t e = entries[i];
         int rank = 0;
+#pragma unroll 8
         for (int j = 0; j < n; j++) rank += entries[j] > e;
         if (rank < top) list[rank] = e;
     }
@@ -784,15 +786,20 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallB
                          remote_float(&sh.all.t, lane)};
             p = join_lanes(p);
             if (kTop) {
-                if (threadIdx.x == 0) sh.found = 0;
-                __syncthreads();
-                for (int i = threadIdx.x; i < cluster * o.top; i += blockDim.x) {
+                const int n = cluster * o.top;
+                for (int i = threadIdx.x; i < n; i += blockDim.x) {
                     const uint64_t* at = &sh.list[i % o.top];
-                    const uint64_t e = (uint64_t)remote((const char*)at + 4, i / o.top) << 32 | remote(at, i / o.top);
-                    if (e) sh.entries[atomicAdd(&sh.found, 1)] = e;
+                    sh.entries[i] = (uint64_t)remote((const char*)at + 4, i / o.top) << 32 | remote(at, i / o.top);
                 }
+                if (threadIdx.x < o.top) sh.joined[threadIdx.x] = 0;
                 __syncthreads();
-                rank_entries(sh.entries, sh.found, o.top, sh.list);
+                for (int i = threadIdx.x; i < n; i += blockDim.x) {
+                    const uint64_t e = sh.entries[i];
+                    int rank = 0;
+#pragma unroll 8
+                    for (int j = 0; j < n; j++) rank += sh.entries[j] > e;
+                    if (e && rank < o.top) sh.joined[rank] = e;
+                }
                 __syncthreads();
             }
         }
@@ -810,7 +817,8 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallB
     const Row r = far ? Row::about_maximum(p) : Row(p, c);
     if (threadIdx.x == 0) write_row(a, o, row, r, act);
     if (kTop)
-        for (int k = threadIdx.x; k < o.top; k += blockDim.x) write_top(o, row, k, sh.list[k], r, a.scale);
+        for (int k = threadIdx.x; k < o.top; k += blockDim.x)
+            write_top(o, row, k, cluster > 1 ? sh.joined[k] : sh.list[k], r, a.scale);
 }
 static_assert(kMaxCluster * B3X_TRAIN_MAX_TOP <= kFound, "the blocks' alternatives are ranked at once");
 
