@@ -657,11 +657,11 @@ __device__ __noinline__ void crowded(const Source<T, kMask>& src, Shared& sh, in
 // from L2.
 //
 // 4,096 rows of 131,072 bf16: 177 us without alternatives (6.1 TB/s, 94% of the
-// copy rate), 219 with 20 (76%).  An exponential a logit keeps the special
+// copy rate), 217 with 20 (77%).  An exponential a logit keeps the special
 // function unit half busy; the rest of the time is the loads' latency at 64
 // registers a thread, and each row's end (sorting, ranking), which other blocks
 // of the SM cover in part.  12 blocks an SM instead of 8 spill (267 us).  8 rows,
-// a cluster of 8 blocks each: 4.6 us without alternatives, 9.8 with 20, all of it
+// a cluster of 8 blocks each: 4.7 us without alternatives, 9.6 with 20, all of it
 // latency.
 template <class T, bool kMask, bool kTop, bool kOnce, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallBlocks) long_kernel(Rows a, Out o, int cluster, int shift) {
@@ -825,7 +825,7 @@ static_assert(kMaxCluster * B3X_TRAIN_MAX_TOP <= kFound, "the blocks' alternativ
 template <class T, bool kMask, bool kTop>
 int launch_long(const Rows& a, const Out& o, int nv, cudaStream_t s) {
     // A cluster a row while rows alone leave SMs idle and each block keeps 1,024 vectors: 8 rows of 131,072 bf16 with 20
-    // alternatives 9.8 us, by single blocks 13.5; 8 rows of 32,768 8.1 us so, by two blocks each 10.2.
+    // alternatives 9.6 us, by single blocks 13.5; 8 rows of 32,768 8.1 us so, by two blocks each 10.2.
     int cluster = 1;
     while (cluster < kMaxCluster && a.rows * cluster * 2 <= 296 && nv / (cluster * 2) >= 1024) cluster *= 2;
     int each = (nv + cluster - 1) / cluster;
