@@ -41,7 +41,11 @@ __device__ __forceinline__ int index_of(uint64_t e) { return (int)(0xFFFFFFFFu -
 //   L = ln s - ln 2 (c m - r),  H = ln s - ln 2 t / s.
 // Joined parts move to the larger r: 2^(x + d) (x + d) = 2^d (2^x x + d 2^x).
 // Shifts and exponents stop at -1e4, where 2^x is 0 already, so that -infinity
-// never meets a zero factor.  A NaN maximum stays; sums beside it mean nothing.
+// never meets a zero factor.  From |c m| = 2^24 on, whole numbers that floats
+// hold are not always near c m: a row with such a maximum is summed about the
+// maximum itself, and a part with one (a stretch filled with -1e9, say), whose
+// sums may be beyond the floats, is dropped where 2^d is 0: in any other row it
+// weighs nothing.  A NaN maximum stays; sums beside it mean nothing.
 struct Part {
     float m, r, s, t;
 };
@@ -51,6 +55,7 @@ __device__ __forceinline__ float reference(float m, float c) { return fminf(fmax
 
 __device__ __forceinline__ Part moved(Part a, float m, float r) {
     const float d = fmaxf(a.r - r, -1e4f), f = exp2_fast(d);
+    if (f == 0.0f) return Part{m, r, 0.0f, 0.0f};   // its sums may be beyond the floats
     return Part{m, r, a.s * f, f * __fmaf_rn(d, a.s, a.t)};
 }
 
@@ -67,9 +72,10 @@ __device__ __forceinline__ Part join_lanes(Part a) {
     return a;
 }
 
-// Whether c m went beyond the floats (logits of 1e38): the row needs sums of (z - m) instead.
-__device__ __forceinline__ bool out_of_range(const Part& a) {
-    return fabsf(a.m) < kInf && !(a.s >= 0.5f && a.s < 1e30f);
+// Whether no whole number is near c m (|c m| of 2^24 and more, or beyond the
+// floats): the row needs sums of (z - m) instead.
+__device__ __forceinline__ bool out_of_range(const Part& a, float c) {
+    return fabsf(a.m) < kInf && !(fabsf(__fmaf_rn(a.m, c, -a.r)) <= 1.0f);
 }
 
 constexpr float kLn2 = 0.6931471805599453f;
@@ -260,8 +266,8 @@ __device__ __forceinline__ int take_equal(const S& src, int v, int v1, uint32_t 
     return min(need, got + all);
 }
 
-// The sums of a row of logits of 1e38, whose products with c are beyond the
-// floats: x = c (z - m).  `by`: threads that share the row.
+// The sums of a row that is out of range: x = c (z - m).  `by`: threads that
+// share the row.
 template <class T, bool kMask>
 __device__ __noinline__ float2 far_sums(const Source<T, kMask>& src, float m, float c, int first, int by) {
     float s = 0.0f, t = 0.0f;
@@ -375,8 +381,8 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 4 : 5) lanes_kernel(Rows a
 #pragma unroll
         for (int k = L / 2; k; k /= 2) p.s += __shfl_xor_sync(~0u, p.s, k), p.t += __shfl_xor_sync(~0u, p.t, k);
     }
-    const bool far = out_of_range(p);
-    if (__any_sync(~0u, far)) {   // logits of 1e38: x = c (z - m)
+    const bool far = out_of_range(p, c);
+    if (__any_sync(~0u, far)) {   // x = c (z - m)
         float s = 0.0f, t = 0.0f;
         for (int v = lane; v < nv; v += L) {
             const uint4 w = src.load(v);
@@ -806,7 +812,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallB
         cluster_sync();   // no block leaves while its shared memory is read
         if (rank) return;
     }
-    const bool far = out_of_range(p);
+    const bool far = out_of_range(p, c);
     if (far) {
         const float2 st = far_sums(src, p.m, c, (int)threadIdx.x, (int)blockDim.x);
         if (lane == 0) sh.far[warp] = st;

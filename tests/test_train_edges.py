@@ -1,0 +1,80 @@
+"""The training operators at values where 32-bit arithmetic can go wrong: large
+negative fills, scales and eps near the ends of the floats, what is no number.
+Tolerances are test_train.py's."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from puffysics_b200 import train
+from test_train import DT, E, INF, built, check_logprob, grad_oracle, host, near, terms_of  # noqa: F401
+
+
+# ---- rows with stretches of a large negative value ---------------------------------------------
+# (fill, scale): products with the scale whose 32-bit neighbours are whole numbers apart, from 8 to beyond the floats
+FILLS = [(-1e7, 1.0), (-1e8, 1.0), (-1e9, 1.0), (-1e9, 1 / 0.6), (-1e9, 2.0), (-2e9, 1 / 1.2), (-2.5e9, 1.0), (-5e9, 1.4),
+         (-5e9, 2.0), (-1e10, 0.7), (-1e10, 1.0), (-1e12, 1.0), (-1e12, 1 / 0.6), (-1e20, 1.0), (-1e30, 2.0), (-1e38, 1 / 0.6)]
+# (rows, width): a warp a row that walks; a block a row in one turn and in several, few rows and many; clusters
+FILLED = [("f32", 1200, 1100), ("bf16", 1200, 2500), ("f32", 40, 4096), ("bf16", 40, 9000), ("bf16", 640, 9000),
+          ("f32", 160, 20000), ("bf16", 8, 131072), ("f32", 3, 300001), ("f32", 50, 400), ("bf16", 50, 30)]
+
+
+def make_filled(rows, width, pad, dtype, fill, seed):
+    """Ordinary logits beside stretches of `fill`: the first places, the last, all but one, every other stretch, all."""
+    rng = np.random.default_rng(seed)
+    z = rng.normal(0, 3, (rows, width))
+    for r in range(rows):
+        kind = r % 6
+        if kind == 0:
+            z[r, :(width * 3) // 20 + 1] = fill
+        elif kind == 1:
+            z[r, width // 2:] = fill
+        elif kind == 2:
+            z[r] = np.where(np.arange(width) == rng.integers(width), z[r], fill)
+        elif kind == 3:
+            z[r, (np.arange(width) // 97) % 2 == 0] = fill
+        elif kind == 4:
+            z[r] = fill
+        else:
+            z[r, rng.random(width) < 0.9] = fill
+    store = torch.full((rows, width + pad), math.nan, dtype=DT[dtype])
+    store[:, :width] = torch.from_numpy(z).to(DT[dtype])
+    return store
+
+
+def check_filled(dtype, rows, width, fill, scale, masked, seed):
+    store = make_filled(rows, width, seed % 3, dtype, fill, seed)
+    rng = np.random.default_rng(seed)
+    actions = torch.from_numpy(rng.integers(0, width, rows))
+    mask = torch.from_numpy((rng.random((rows, width)) < 0.8).astype(np.uint8)) if masked else None
+    dev, act, dmask, out, want = check_logprob(store, width, actions, mask, scale, 0)
+    g, h = rng.normal(0, 1, rows).astype(np.float32), rng.normal(0, 1, rows).astype(np.float32)
+    grad = torch.full((rows, width), 7.0, device="cuda")
+    assert train.logprob_grad(dev[:, :width].float(), out["stats"], grad, actions=act, mask=dmask, scale=scale,
+                              d_logp=torch.from_numpy(g).cuda(), entropy=out["entropy"], d_entropy=torch.from_numpy(h).cuda()) == 0
+    want_g, size = grad_oracle(store[:, :width].double().numpy(), want, actions.numpy(), mask, scale, g, h)
+    n, total = terms_of(width), want["stats"][:, 1:]
+    tol = size * E * 2 * (n + 80) * (1 + total) + np.abs(h[:, None]) * scale * np.exp(want["lp"]) * E * (n + 64) * (2 + 2 * total)
+    near(grad.cpu().numpy(), want_g, tol * (1 + E) + np.abs(want_g) * E + 2.0 ** -149 + 1e-30)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype,rows,width", FILLED)
+def test_logprob_and_gradient_of_filled_rows(dtype, rows, width, masked):
+    """A large negative value in the place of logits that are not allowed is a value like any other: log
+    probabilities, entropy and gradient stay those of the formula, whichever threads' places are all filled."""
+    some = FILLS if rows * width < 400000 else FILLS[FILLED.index((dtype, rows, width)) % 3 + masked::4]
+    for k, (fill, scale) in enumerate(some):
+        check_filled(dtype, rows, width, fill, scale, masked, k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,width", [(1200, 2500), (40, 9000), (8, 131072)])
+def test_logprob_of_filled_rows_in_half_precision(rows, width):
+    """The same by the scale: -60,000 at 1e5, logits of some 1e-5 beside it."""
+    scale = 1e5
+    store = make_filled(rows, width, 1, "f32", -6e9, 1)
+    store = (store.double() / scale).to(torch.float16)
+    check_logprob(store, width, torch.from_numpy(np.random.default_rng(1).integers(0, width, rows)), None, scale, 0)
