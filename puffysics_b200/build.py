@@ -123,8 +123,14 @@ def train_cmd(extra=()):
             + list(extra) + TRAIN_SRC + ["-o", TRAIN_LIB])
 
 
+def torch_dir():
+    """Where torch is installed (not imported: that takes seconds), or None."""
+    spec = importlib.util.find_spec("torch")
+    return spec.submodule_search_locations[0] if spec else None
+
+
 def train_py_cmd():
-    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    torch = torch_dir()
     include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"]]
     libs = os.path.join(torch, "lib")
@@ -134,9 +140,18 @@ def train_py_cmd():
                "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + libs, "-o", TRAIN_PY_LIB])
 
 
+def train_py_up_to_date():
+    """Whether the training operators' Python side is built, or has no torch to be built against."""
+    return torch_dir() is None or not _newer(TRAIN_PY_LIB, [TRAIN_PY_SRC, TRAIN_HEADERS[0], __file__])
+
+
 def build_train_py(force=False):
-    """The training operators' Python side (after libb3train.so, which it links)."""
-    if not force and not _newer(TRAIN_PY_LIB, [TRAIN_PY_SRC, TRAIN_HEADERS[0], __file__]):
+    """The training operators' Python side (after libb3train.so, which it
+    links).  The C-ABI libraries need no torch: without it this one is left out."""
+    if torch_dir() is None:
+        sys.stderr.write("%s left out: no torch here\n" % os.path.basename(TRAIN_PY_LIB))
+        return
+    if not force and train_py_up_to_date():
         return
     cmd = train_py_cmd()
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -183,8 +198,7 @@ def up_to_date():
     return (not _newer(LIB, deps) and not any(_newer(scenes_lib(n), [SCENES_SRC] + HEADERS) for n in SCENE_CONFIGS)
             and not any(_newer(thread_lib(n), thread_deps) for n in thread_lib_names())
             and not _newer(HOVER_LIB, [HOVER_SRC, __file__] + THREAD_DEPS + HOVER_HEADERS)
-            and not _newer(TRAIN_LIB, TRAIN_SRC + TRAIN_HEADERS + [__file__])
-            and not _newer(TRAIN_PY_LIB, [TRAIN_PY_SRC, TRAIN_HEADERS[0], __file__]))
+            and not _newer(TRAIN_LIB, TRAIN_SRC + TRAIN_HEADERS + [__file__]) and train_py_up_to_date())
 
 
 def build_scenes(force=False):
@@ -211,15 +225,14 @@ def build(force=False, verbose=False):
     os.makedirs(LIB_DIR, exist_ok=True)
     build_scenes(force)
     build_thread_libs(force)
-    build_train_py(force)
-    if not force and not _newer(LIB, SOURCES + HEADERS + [__file__]):
-        return LIB
-    cmd = nvcc_cmd(extra=["-Xptxas", "-v"] if verbose else [])
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
-    if verbose:
-        sys.stdout.write(res.stdout + res.stderr)
+    if force or _newer(LIB, SOURCES + HEADERS + [__file__]):
+        cmd = nvcc_cmd(extra=["-Xptxas", "-v"] if verbose else [])
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + " ".join(cmd) + "\n" + res.stdout + res.stderr)
+        if verbose:
+            sys.stdout.write(res.stdout + res.stderr)
+    build_train_py(force)   # last: what goes wrong with torch leaves the other libraries built
     return LIB
 
 
