@@ -9,6 +9,7 @@ rounds exactly like the reference's CPU build with -ffp-contract=off.
 """
 import importlib.util
 import os
+import re
 import subprocess
 import sys
 import sysconfig
@@ -129,20 +130,36 @@ def torch_dir():
     return spec.submodule_search_locations[0] if spec else None
 
 
+def torch_version():
+    with open(os.path.join(torch_dir(), "version.py")) as f:
+        return re.search(r"__version__ = ['\"]([^'\"]+)", f.read()).group(1)
+
+
+def built_for():
+    """What the training operators' Python side is compiled against; the library holds these words."""
+    return "b3train_py built for torch %s, %s" % (torch_version(), sysconfig.get_config_var("SOABI"))
+
+
+def train_py_current():
+    """Whether the library there is was compiled against the torch and Python that are here."""
+    with open(TRAIN_PY_LIB, "rb") as f:
+        return built_for().encode() + b"\0" in f.read()
+
+
 def train_py_cmd():
     torch = torch_dir()
     include = [os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"]]
     libs = os.path.join(torch, "lib")
     return ([CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden"]
-            + [x for d in include for x in ("-isystem", d)] + ["-I" + os.path.join(ROOT, "include"), TRAIN_PY_SRC,
+            + [x for d in include for x in ("-isystem", d)] + ["-I" + os.path.join(ROOT, "include"), '-DB3X_BUILT_FOR="%s"' % built_for(), TRAIN_PY_SRC,
                "-L" + LIB_DIR, "-lb3train", "-L" + libs, "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10",
                "-Wl,-rpath,$ORIGIN", "-Wl,-rpath," + libs, "-o", TRAIN_PY_LIB])
 
 
 def train_py_up_to_date():
     """Whether the training operators' Python side is built, or has no torch to be built against."""
-    return torch_dir() is None or not _newer(TRAIN_PY_LIB, [TRAIN_PY_SRC, TRAIN_HEADERS[0], __file__])
+    return torch_dir() is None or (not _newer(TRAIN_PY_LIB, [TRAIN_PY_SRC, TRAIN_HEADERS[0], __file__]) and train_py_current())
 
 
 def build_train_py(force=False):

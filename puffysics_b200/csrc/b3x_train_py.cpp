@@ -13,6 +13,9 @@
 
 #include "b3x_train.h"
 
+// The torch and Python that this is compiled against (the build compares).
+extern "C" __attribute__((visibility("default"))) const char b3train_py_built_for[] = B3X_BUILT_FOR;
+
 namespace {
 
 constexpr int kInvalid = 1;   // cudaErrorInvalidValue

@@ -23,6 +23,8 @@ import os
 
 import torch
 
+from . import build
+
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "_lib", "libb3train.so")
 PY_PATH = os.path.join(_PKG, "_lib", "b3train_py.so")
@@ -64,6 +66,8 @@ def _binding():
     if _py is None:
         if not os.path.exists(PY_PATH):
             raise RuntimeError("%s is not built; run python -m puffysics_b200.build" % PY_PATH)
+        if not build.train_py_current():
+            raise RuntimeError("%s is not %s; run python -m puffysics_b200.build" % (PY_PATH, build.built_for()))
         spec = importlib.util.spec_from_file_location("b3train_py", PY_PATH)
         _py = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(_py)

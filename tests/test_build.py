@@ -39,3 +39,16 @@ def test_the_step_library_builds_beside_a_torch_that_does_not_compile(commands):
     with pytest.raises(RuntimeError, match="no such header"):
         build.build()
     assert has(commands, build.LIB) and has(commands, build.TRAIN_PY_LIB)
+
+
+def test_the_torch_side_follows_the_installed_torch(monkeypatch):
+    """A library built against another torch's headers is stale for the build, and not loaded."""
+    from puffysics_b200 import train
+    build.build()
+    assert build.train_py_up_to_date() and train._binding()
+    assert build.torch_version() in build.built_for()
+    monkeypatch.setattr(build, "torch_version", lambda: "99.0")
+    assert not build.train_py_up_to_date() and not build.up_to_date()
+    monkeypatch.setattr(train, "_py", None)
+    with pytest.raises(RuntimeError, match="99.0"):
+        train._binding()
