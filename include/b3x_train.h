@@ -91,7 +91,9 @@ B3X_TRAIN_API int b3x_train_logprob_grad_gpu(const void* logits, int type, long 
  *   A_t = delta_t + gamma lam n_t A_{t+1},     R_t = A_t + v_t
  *
  * v after the last step is last_values.  A terminal step takes nothing from
- * beyond it, NaN included.  lengths (NULL: all `steps`) gives each
+ * beyond it, NaN included, and with a gamma lam of 0 in 32 bits no step takes
+ * anything from a later advantage; else a NaN or infinity reaches every step
+ * before it.  lengths (NULL: all `steps`) gives each
  * environment's number of steps; last_values follow the last of them, and
  * advantages and returns beyond are 0 whatever the inputs hold there (a length
  * outside [0, steps] counts as the nearer end).  values and last_values have

@@ -1,15 +1,18 @@
 // b3x_train_advantage.cu -- generalised advantages and returns of a rollout
 // (b3x_train.h).
 //
-// A_t = x_t + a_t A_{t+1} with x_t = delta_t and a_t = gamma lam, or 0 where the
-// step ends an episode or is an environment's last.  Steps in a row compose to
+// A_t = x_t + a_t A_{t+1} with x_t = delta_t and a_t = gamma lam, or nothing
+// after x_t where the step ends an episode or is an environment's last: a_t is
+// NaN there, which any product with it stays.  Steps in a row compose to
 // a pair (a, b) too, A = b + a A_after, and pairs compose associatively; so time
 // is split over threads: each composes a few consecutive steps in registers, a
 // suffix scan over lanes, warps and blocks gives each thread the A after its
 // steps, and it walks back through them.  Inputs are read once and outputs
 // written once; bound by memory for large rollouts and by the launch and one
-// trip to memory for those of an environment batch.  Where a is 0 nothing is
-// multiplied: what lies beyond a terminal may be NaN.
+// trip to memory for those of an environment batch.  Where a is NaN nothing is
+// multiplied: what lies beyond a terminal may be NaN itself.  A product of many
+// gamma lam never becomes 0: a NaN or infinity reaches every step before it,
+// back to a terminal, however the steps are split.
 #include <cmath>
 
 #include "b3x_train_common.cuh"
@@ -25,19 +28,27 @@ struct Rollout {
     const int* lengths;
     float *advantages, *returns;
     long long rt, rn, vt, vn, dt, dn, ln, at, an, ot, on;
-    float gamma, decay;  // gamma, gamma * lam
+    float gamma, decay;  // gamma, gamma * lam (kCut where that is 0)
 };
 
-// A = b + a A_after.
+constexpr float kCut = __builtin_nanf("");
+
+// A = b + a A_after, or b where a is NaN.
 struct Pair {
     float a, b;
 };
-__device__ __forceinline__ float apply(Pair p, float after) { return p.a != 0.0f ? __fmaf_rn(p.a, after, p.b) : p.b; }
-__device__ __forceinline__ Pair compose(Pair first, Pair then) { return Pair{first.a * then.a, apply(first, then.b)}; }
+__device__ __forceinline__ float apply(Pair p, float after) { return p.a == p.a ? __fmaf_rn(p.a, after, p.b) : p.b; }
+// A product that fell to 0 becomes the least of the floats.
+__device__ __forceinline__ float not_zero(float a) {
+    float y;
+    asm("max.NaN.xorsign.abs.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(0x1p-149f));
+    return y;
+}
+__device__ __forceinline__ Pair compose(Pair first, Pair then) { return Pair{not_zero(first.a * then.a), apply(first, then.b)}; }
 
 // kSteps consecutive steps of one environment, from t on.  A step outside the
 // rollout leaves A as it is (a = 1, x = 0); one beyond its environment's end has
-// A = 0 (a = 0, x = 0).
+// A = 0 (a = kCut, x = 0).
 template <int kSteps>
 struct Steps {
     float x[kSteps], a[kSteps], v[kSteps];
@@ -45,7 +56,8 @@ struct Steps {
     __device__ __forceinline__ Pair pair() const {
         Pair p{a[kSteps - 1], x[kSteps - 1]};
 #pragma unroll
-        for (int i = kSteps - 2; i >= 0; i--) p = compose(Pair{a[i], x[i]}, p);
+        for (int i = kSteps - 2; i >= 0; i--) p = Pair{a[i] * p.a, apply(Pair{a[i], x[i]}, p.b)};
+        p.a = not_zero(p.a);
         return p;
     }
 };
@@ -98,23 +110,23 @@ __device__ __forceinline__ Steps<kSteps> load_steps(const Rollout& a, int n, int
         for (int i = 0; i < kSteps; i++) {
             const float next = i == kSteps - 1 ? after : s.v[i + 1];
             s.x[i] = (end[i] ? s.x[i] : __fmaf_rn(a.gamma, next, s.x[i])) - s.v[i];
-            s.a[i] = end[i] ? 0.0f : a.decay;
+            s.a[i] = end[i] ? kCut : a.decay;
         }
-        if (t + kSteps == len) s.a[kSteps - 1] = 0.0f;
+        if (t + kSteps == len) s.a[kSteps - 1] = kCut;
         return s;
     }
 #pragma unroll
     for (int i = 0; i < kSteps; i++) {
         const int k = t + i;
         s.x[i] = s.v[i] = 0.0f;
-        s.a[i] = k >= 0 && k < a.steps ? 0.0f : 1.0f;
+        s.a[i] = k >= 0 && k < a.steps ? kCut : 1.0f;
         if (k >= 0 && k < len) {
             const float next = k + 1 < len ? to_float(v[(long long)(i + 1) * a.vt]) : to_float(((const V*)a.last_values)[n * a.ln]);
             const bool over = d[(long long)i * a.dt] != (D)0;
             s.v[i] = to_float(v[(long long)i * a.vt]);
             s.x[i] = r[(long long)i * a.rt];
             s.x[i] = (over ? s.x[i] : __fmaf_rn(a.gamma, next, s.x[i])) - s.v[i];
-            s.a[i] = over || k + 1 == len ? 0.0f : a.decay;
+            s.a[i] = over || k + 1 == len ? kCut : a.decay;
         }
     }
     return s;
@@ -352,7 +364,7 @@ int b3x_train_advantage_gpu(long long steps, long long envs, const float* reward
         return (int)cudaErrorInvalidValue;
     const Rollout a{(int)steps, (int)envs, rewards, values, terminals, last_values, lengths, advantages, returns,
                     strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], strides[6],
-                    strides[7], strides[8], strides[9], strides[10], gamma, gamma * lam};
+                    strides[7], strides[8], strides[9], strides[10], gamma, gamma * lam != 0.0f ? gamma * lam : kCut};
     // 4 steps at a time: consecutive in memory, every array's rows at the same place among groups of 4
     const auto place = [](const void* p, int bytes) { return (uintptr_t)p / bytes % 4; };
     bool vec = steps > 1 && strides[0] == 1 && strides[2] == 1 && strides[4] == 1 && strides[7] == 1 &&

@@ -78,3 +78,27 @@ def test_logprob_of_filled_rows_in_half_precision(rows, width):
     store = make_filled(rows, width, 1, "f32", -6e9, 1)
     store = (store.double() / scale).to(torch.float16)
     check_logprob(store, width, torch.from_numpy(np.random.default_rng(1).integers(0, width, rows)), None, scale, 0)
+
+
+# ---- what is no number, far ahead ---------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["time", "env"])
+@pytest.mark.parametrize("steps,envs", [(20, 5), (100, 64), (9000, 3), (4000, 40), (3000, 700), (300, 9000), (65536, 1)])
+@pytest.mark.parametrize("gamma,lam", [(0.99, 0.95), (0.9, 0.1), (1.0, 1e-30), (-0.9, 0.1)])
+def test_advantage_carries_nan_and_infinity_to_every_earlier_step(steps, envs, order, gamma, lam):
+    """What is no number at a step reaches every step before it back to a terminal, however far and in every layout:
+    a product of many gamma lam is below the floats, but it is not the 0 of a terminal."""
+    def lay(x):
+        return x.cuda() if order == "time" else x.t().contiguous().cuda().t()
+    r, v, d = (torch.zeros((steps, envs)) for _ in range(3))
+    r += 1
+    r[steps - 1, 0::3] = math.nan
+    r[steps - 1, 1::3] = INF
+    cut = steps // 2
+    d[cut, 1::3] = 1          # from the step after the terminal on
+    adv = lay(torch.full((steps, envs), 7.0))
+    assert train.advantage(lay(r), lay(v), lay(d), torch.zeros(envs, device="cuda"), adv, gamma=gamma, lam=lam) == 0
+    got = adv.cpu()
+    assert torch.isnan(got[:, 0::3]).all()
+    assert torch.isinf(got[cut + 1:, 1::3]).all() and torch.isfinite(got[:cut + 1, 1::3]).all()
+    assert torch.isfinite(got[:, 2::3]).all()
