@@ -600,9 +600,12 @@ int b3x_train_adamw_gpu(int count, void* const* params, int param_type, const vo
             return (int)cudaErrorInvalidValue;
     }
     const double t = (double)step;
+    // The reciprocal of sqrt(v) root + eps takes numbers under the normal floats for 0: where eps is near those, both
+    // terms and the rate are 2^24 times as large.
+    const float up = (float)eps > 0.0f && (float)eps < 0x1p-100f ? 0x1p24f : 1.0f;
     const Hyper h{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2),
-                  (float)(lr / (1.0 - std::pow(beta1, t))), (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, t))),
-                  (float)eps, grad_scale};
+                  (float)(lr / (1.0 - std::pow(beta1, t))) * up, (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, t))) * up,
+                  (float)eps * up, grad_scale};
     const cudaStream_t s = (cudaStream_t)stream;
     auto fill = [&](int k) {
         const double wd = decays ? (double)decays[k] : weight_decay;

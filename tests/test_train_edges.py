@@ -102,3 +102,25 @@ def test_advantage_carries_nan_and_infinity_to_every_earlier_step(steps, envs, o
     assert torch.isnan(got[:, 0::3]).all()
     assert torch.isinf(got[cut + 1:, 1::3]).all() and torch.isfinite(got[:cut + 1, 1::3]).all()
     assert torch.isfinite(got[:, 2::3]).all()
+
+
+# ---- eps below the normal floats -----------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("state", ["f32", "f8"])
+@pytest.mark.parametrize("eps", [1e-40, 2e-38, 1e-30])
+def test_adamw_tiny_eps(eps, state):
+    """eps below the normal floats: an element without a gradient stays where it is, one whose squared gradient is
+    below the floats takes the formula's step."""
+    n = 600
+    p0 = np.random.default_rng(0).normal(0, 1, n).astype(np.float32)
+    grads = np.zeros(n, np.float32)
+    grads[300:400] = 1e-25 if state == "f32" else 0.0
+    p, g = torch.from_numpy(p0.copy()).cuda(), torch.from_numpy(grads).cuda()
+    kind = torch.float32 if state == "f32" else torch.float8_e4m3fn
+    m, v = (torch.zeros(n, device="cuda").to(kind) for _ in range(2))
+    sc = [torch.zeros((3, 2), device="cuda")] if state == "f8" else None
+    lr = float(np.float32(eps)) * 1e20      # steps of about 1e-5
+    assert train.adamw([p], [g], [m], [v], 1, lr, 0.9, 0.95, eps, 0.0, scales=sc) == 0
+    mm = (grads * np.float32(1 - 0.9)).astype(np.float64)
+    size = lr * (mm / (1 - 0.9)) / float(np.float32(eps))
+    near(host(p), p0 - size, E * (4 * np.abs(p0) + 13 * np.abs(size)) + 1e-40)
