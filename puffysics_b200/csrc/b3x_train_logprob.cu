@@ -33,6 +33,10 @@ __device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t index) {
 }
 __device__ __forceinline__ int index_of(uint64_t e) { return (int)(0xFFFFFFFFu - (uint32_t)e); }
 
+// scale log2 e, within the floats for any finite scale: from 2.4e38 on only a
+// row's maximum has a probability, with that factor as with the largest float.
+__device__ __forceinline__ float factor_of(const Rows& a) { return fminf(a.scale * kLog2e, 3.402823466e38f); }
+
 // ---- running sums -----------------------------------------------------------------------
 // What a part of a row comes to: its maximum m, a whole number r near c m
 // (c = scale log2 e), s = sum 2^x and t = sum x 2^x with x = c z - r.  r is
@@ -150,7 +154,7 @@ __global__ void __launch_bounds__(kShortThreads) short_kernel(Rows a, Out o) {
         z[i] = i < a.width ? logit<T>(a, row, i) : -kInf;
         p.m = max_nan(p.m, z[i]);
     }
-    const float c = a.scale * kLog2e;
+    const float c = factor_of(a);
 #pragma unroll
     for (int i = 0; i < kShort; i++) {   // the maximum is known before the sums: x = c (z - m)
         const float x = fmaxf((z[i] - p.m) * c, -1e4f), e = exp2_fast(x);
@@ -343,7 +347,7 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 4 : 5) lanes_kernel(Rows a
     const bool on = row < a.rows;
     const Source<T, kMask, kTop> src(a, on ? row : 0);
     const int nv = on ? src.vectors() : 0;
-    const float c = a.scale * kLog2e;
+    const float c = factor_of(a);
     if (kTop && lane == 0) found[here] = 0;
     Action act{false, 0.0f};
     if (on && lane == 0) act = load_action<T>(a, o, row);
@@ -679,7 +683,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallB
     const int nv = src.vectors();
     const int each = ((nv + cluster - 1) / cluster + (1 << shift) - 1) >> shift << shift;
     const int v0 = min(nv, each * rank), v1 = min(nv, v0 + each);
-    const float c = a.scale * kLog2e;
+    const float c = factor_of(a);
     if (kTop) {
         if (!kOnce)
             for (int i = threadIdx.x; i < kGroups; i += blockDim.x) sh.group[i] = 0;

@@ -124,3 +124,17 @@ def test_adamw_tiny_eps(eps, state):
     mm = (grads * np.float32(1 - 0.9)).astype(np.float64)
     size = lr * (mm / (1 - 0.9)) / float(np.float32(eps))
     near(host(p), p0 - size, E * (4 * np.abs(p0) + 13 * np.abs(size)) + 1e-40)
+
+
+# ---- scales near the ends of the floats ----------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [2.0 ** -140, 1e-30, 1e30, 3.0e38])
+@pytest.mark.parametrize("dtype,rows,width", [("f32", 9, 5), ("f32", 9, 40), ("bf16", 9, 700), ("f32", 1200, 1100), ("f32", 9, 5000),
+                                              ("bf16", 8, 131072)])
+def test_logprob_of_any_finite_scale(dtype, rows, width, scale):
+    """Scales near both ends of the floats: with 3e38 its product with log2(e) is beyond them.  Equal logits have
+    probability 1 / width whatever the scale, and a row's lone largest logit has 1 at a large one."""
+    z = torch.zeros((rows, width + 3), dtype=DT[dtype])
+    z[1::3, width // 2] = 2.0
+    z[2::3] = -1.5
+    check_logprob(z, width, torch.full((rows,), width // 2), None, scale, 0)
