@@ -33,7 +33,7 @@ const at::Tensor* tensor(PyObject* o) {
 }
 
 const at::Tensor& here(const at::Tensor* t, int64_t device) {
-    require(t && t->is_cuda() && t->get_device() == device && t->layout() == at::kStrided);
+    require(t && t->is_cuda() && t->get_device() == device && t->layout() == at::kStrided && !t->is_neg());
     return *t;
 }
 

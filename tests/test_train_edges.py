@@ -138,3 +138,21 @@ def test_logprob_of_any_finite_scale(dtype, rows, width, scale):
     z[1::3, width // 2] = 2.0
     z[2::3] = -1.5
     check_logprob(z, width, torch.full((rows,), width // 2), None, scale, 0)
+
+
+# ---- views that torch negates lazily -------------------------------------------------------------
+@pytest.mark.gpu
+def test_lazily_negated_views_are_refused():
+    """The imaginary part of a conjugate is a view whose memory holds the values with the other sign."""
+    z = torch.view_as_complex(torch.ones((6, 4, 2), device="cuda"))
+    neg = z.conj().imag
+    assert neg.is_neg() and (neg == -1).all()
+    plain, last, adv = torch.ones((6, 4), device="cuda"), torch.zeros(4, device="cuda"), torch.full((6, 4), 7.0, device="cuda")
+    for at in range(3):
+        args = [plain, plain.clone(), torch.zeros_like(plain)]
+        args[at] = neg
+        assert train.advantage(*args, last, adv) == 1
+    assert train.advantage(plain, plain.clone(), torch.zeros_like(plain), last, neg) == 1
+    assert (adv == 7).all() and (neg == -1).all()
+    assert train.advantage(neg.resolve_neg(), plain, torch.zeros_like(plain), last, adv) == 0
+    torch.cuda.synchronize()
