@@ -62,6 +62,22 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     return r;
 }
 
+// Square roots of two numbers in [2^-96, 2^100], rounded as sqrtf rounds them:
+// Newton's step from s = v y, y an approximate 1 / sqrt(v), with the residual
+// v - s^2 formed by a fused operation (Markstein 1990).  What is left of the
+// error before the last rounding, about 2^-45, decides no rounding of a 24-bit
+// number (the tests compare all significands of two octaves with sqrtf).
+// sqrtf's own cases for other numbers cost a branch a number.
+__device__ __forceinline__ uint64_t sqrt2(uint64_t v) {
+    const float2 x = unpack2(v);
+    float2 y;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.x) : "f"(x.x));
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(y.y) : "f"(x.y));
+    const uint64_t y2 = pack2(y.x, y.y), s = mul2(v, y2), minus = mul2(s, pack2(-1.0f, -1.0f));
+    const uint64_t half = mul2(y2, pack2(0.5f, 0.5f));
+    return fma2(fma2(minus, s, v), half, s);
+}
+
 // Whether (rows, cols) elements at these strides are apart from one another.
 inline bool apart(long long rows, long long cols, long long rs, long long cs) {
     if (rows < 2 && cols < 2) return true;

@@ -1,13 +1,16 @@
 """The training operators at values where 32-bit arithmetic can go wrong: large
 negative fills, scales and eps near the ends of the floats, what is no number.
 Tolerances are test_train.py's."""
+import ctypes
 import math
+import os
+import subprocess
 
 import numpy as np
 import pytest
 import torch
 
-from puffysics_b200 import train
+from puffysics_b200 import build, train
 from test_train import DT, E, INF, built, check_logprob, grad_oracle, host, near, terms_of  # noqa: F401
 
 
@@ -156,3 +159,40 @@ def test_lazily_negated_views_are_refused():
     assert (adv == 7).all() and (neg == -1).all()
     assert train.advantage(neg.resolve_neg(), plain, torch.zeros_like(plain), last, adv) == 0
     torch.cuda.synchronize()
+
+
+# ---- square roots ------------------------------------------------------------------------------
+SQRT = r"""
+#include "b3x_train_common.cuh"
+__global__ void compare(float up, int* bad) {   // all floats of [1, 4), times a power of 4
+    for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < 1 << 24; i += gridDim.x * blockDim.x) {
+        const float x = __uint_as_float(0x3F800000u + i) * up, y = __uint_as_float(0x3F800000u + ((i + 1) & 0xFFFFFF)) * up;
+        const float2 r = b3t::unpack2(b3t::sqrt2(b3t::pack2(x, y)));
+        if (r.x != sqrtf(x) || r.y != sqrtf(y)) atomicAdd(bad, 1);
+    }
+}
+extern "C" __attribute__((visibility("default"))) int differing(float up, int* bad) {
+    compare<<<1024, 256>>>(up, bad);
+    const cudaError_t e = cudaGetLastError();
+    return e != cudaSuccess ? (int)e : (int)cudaDeviceSynchronize();
+}
+"""
+
+
+@pytest.mark.gpu
+def test_square_roots_of_the_moments_are_those_of_sqrtf(tmp_path):
+    """Every significand of two octaves, at both ends of the range and in between."""
+    src, lib = tmp_path / "sqrt.cu", tmp_path / "libsqrt.so"
+    src.write_text(SQRT)
+    cmd = ([build.NVCC] + build.ARCH + ["-O3", "-std=c++17"] + build.PARITY
+           + ["-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-cudart", "static", "-I" + os.path.join(build.ROOT, "include"),
+              "-I" + os.path.join(build.PKG, "csrc"), str(src), "-o", str(lib)])
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    assert res.returncode == 0, res.stdout + res.stderr
+    f = ctypes.CDLL(str(lib)).differing
+    f.argtypes = [ctypes.c_float, ctypes.c_void_p]
+    for up in (-96, -50, 0, 40, 98):
+        bad = torch.zeros(1, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        assert f(2.0 ** up, bad.data_ptr()) == 0
+        assert int(bad) == 0, up
