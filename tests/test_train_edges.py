@@ -11,7 +11,8 @@ import pytest
 import torch
 
 from puffysics_b200 import build, train
-from test_train import DT, E, INF, built, check_logprob, grad_oracle, host, near, terms_of  # noqa: F401
+from test_train import (DT, E, H, INF, built, check_logprob, grad_oracle, host, make_adam, near, np_decode,  # noqa: F401
+                        np_mix, np_pack, terms_of)
 
 
 # ---- rows with stretches of a large negative value ---------------------------------------------
@@ -196,3 +197,82 @@ def test_square_roots_of_the_moments_are_those_of_sqrtf(tmp_path):
         torch.cuda.synchronize()
         assert f(2.0 ** up, bad.data_ptr()) == 0
         assert int(bad) == 0, up
+
+
+# ---- AdamW: parameters of long lists, copies beside stochastic rounding ------------------------------
+def low_bits(index, tensor, step, seed):
+    """The 16 random bits that round a bfloat16 parameter, and the 32 of its moments."""
+    M = np.uint64(0xFFFFFFFF)
+    key = np_mix(np.array([(seed + tensor * 0x9E3779B1 + step * 0x6A09E667) & 0xFFFFFFFF], np.uint64))[0]
+    bits = np_mix(((index & M) * np.uint64(0x9E3779B1) + (index >> np.uint64(32)) * np.uint64(0x6A09E667) + key) & M)
+    return np_mix((bits + np.uint64(0x9E3779B1)) & M) & np.uint64(0xFFFF), bits
+
+
+def check_rounded(got, want, tol, low=None):
+    """bfloat16 numbers: the 32-bit result, within tol of want, plus its random bits and cut, or rounded to nearest.
+    Either way a larger result never gives a smaller number."""
+    def rounded(x):
+        if low is None:
+            return torch.from_numpy(x).float().to(torch.bfloat16).float().numpy()
+        return ((x.astype(np.float32).view(np.uint32) + low.astype(np.uint32)) & np.uint32(0xFFFF0000)).view(np.float32)
+    bad = np.isnan(want)      # an infinite gradient
+    assert np.array_equal(np.isnan(got), bad)
+    assert ((rounded(want - tol) <= got) & (got <= rounded(want + tol)) | bad).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("param,grad,state,seed", [("f32", "f32", "f32", None), ("f32", "bf16", "f8", 7), ("bf16", "bf16", "f32", 7),
+                                                   ("bf16", "bf16", "f8", 7), ("bf16", "f16", "f8", None)])
+def test_adamw_parameters_of_millions(param, grad, state, seed):
+    """Chunks of several turns: parameters against the formula in 64 bits, from the moments in 32; copies are the
+    32-bit results rounded to nearest, also where the parameters are rounded stochastically."""
+    sizes, step = [10000001, 37, 300000], 3
+    s = make_adam(sizes, param, grad, state, 3)
+    before = {k: None if v is None else [host(t).copy() for t in v] for k, v in s.items() if k != "whole"}
+    copies = [torch.zeros(n, dtype=torch.bfloat16, device="cuda") for n in sizes]
+    decays = [0.1, 0.0, 0.2]
+    assert train.adamw(s["params"], s["grads"], s["m"], s["v"], step, weight_decay=decays, scales=s["scales"], copies=copies,
+                       seed=seed, **H) == 0
+    b1, c1, b2, c2 = (np.float32(x) for x in (0.9, 1 - 0.9, 0.95, 1 - 0.95))
+    for k, n in enumerate(sizes):
+        g, m, v = before["grads"][k], before["m"][k], before["v"][k]
+        if state == "f8":
+            sc = before["scales"][k].repeat(256, 0)[:n]
+            m, r = np_decode(m) * sc[:, 0], np_decode(v) * sc[:, 1]
+            v = r * r
+        m, v = (m * b1 + g * c1).astype(np.float64), (v * b2 + (g * g) * c2).astype(np.float64)
+        p = before["params"][k].astype(np.float64)
+        with np.errstate(invalid="ignore"):
+            size = H["lr"] * (m / (1 - 0.9 ** step)) / (np.sqrt(v / (1 - 0.95 ** step)) + H["eps"])
+        want = p * (1 - H["lr"] * np.float64(np.float32(decays[k]))) - size
+        tol = E * (3 * np.abs(p) + 12 * np.abs(size) + np.abs(want)) + 1e-40
+        got = host(s["params"][k])
+        check_rounded(host(copies[k]), want, tol)
+        if param == "f32":
+            near(got, want, tol)
+            assert torch.equal(copies[k], s["params"][k].to(torch.bfloat16))
+        elif seed is None:
+            assert torch.equal(copies[k].view(torch.int16), s["params"][k].view(torch.int16))
+        else:
+            check_rounded(got, want, tol, low_bits(np.arange(n, dtype=np.uint64), k, step, seed)[0])
+
+
+@pytest.mark.gpu
+def test_adamw_moments_and_parameters_beyond_32_bits():
+    """The last elements of a tensor of 2^32 + 700: codes of sqrt(v) bit for bit, parameters by their random bits."""
+    n, tail, seed, lr = (1 << 32) + 700, 1000, 11, 1e-2
+    p, g = (torch.zeros(n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    m, v = (torch.zeros(n, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn) for _ in range(2))
+    sc = torch.zeros(((n + 255) // 256, 2), device="cuda")
+    first = (n - tail) // 256 * 256
+    g[first:] = torch.from_numpy(np.random.default_rng(0).normal(0, 1, n - first).astype(np.float32)).cuda()
+    grads = host(g[first:])
+    assert train.adamw([p], [g], [m], [v], 1, lr, scales=[sc], weight_decay=0.0, seed=seed) == 0
+    low, bits = low_bits(np.arange(first, n, dtype=np.uint64), 0, 1, seed)
+    root = np.sqrt((grads * grads) * np.float32(1 - 0.999))
+    cv, sv = np_pack(root, bits >> np.uint64(16))
+    cv = np.where((cv == 0) & (root > 0) & (sv.repeat(256)[:len(root)] > 0), 1, cv)
+    assert np.array_equal(host(v[first:]), cv) and np.array_equal(host(sc[first // 256:, 1]), sv)
+    mm = (grads * np.float32(1 - 0.9)).astype(np.float64)
+    want = -lr * (mm / (1 - 0.9)) / (root.astype(np.float64) / math.sqrt(1 - 0.999) + 1e-8)
+    check_rounded(host(p[first:]), want, 12 * E * np.abs(want) + 1e-40, low)
