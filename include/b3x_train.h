@@ -79,7 +79,8 @@ B3X_TRAIN_API int b3x_train_logprob_gpu(const void* logits, int type, long long 
  * and may be the logits themselves (same pointer and stride), not overlap them
  * otherwise.  d_logp or d_entropy (with entropy) may be NULL: zero.  An action
  * that is "none" or has probability 0 by its mask or -infinity takes no
- * d_logp; masked places get 0.  Rounded once, to nearest. */
+ * d_logp; masked places get 0.  Rounded once, to nearest.  Fastest where a row
+ * of grad lies at the same place modulo 16 bytes as its logits. */
 B3X_TRAIN_API int b3x_train_logprob_grad_gpu(const void* logits, int type, long long rows, long long width,
         long long row_stride, const unsigned char* mask, long long mask_stride, const void* actions,
         int action_bytes, float scale, const float* stats, const float* entropy, const float* d_logp,
@@ -122,7 +123,11 @@ B3X_TRAIN_API int b3x_train_grad_norm_gpu(int count, const void* const* grads, i
  *   g = grad grad_scale[0];  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  *
- * in 32 bits, each operation rounded.  params: B3X_F32 or B3X_BF16; grads:
+ * in 32 bits.  For m, v and the square root every operation rounds by itself, so
+ * moments, codes and scales are the formula's bits; the parameter is within a few
+ * units in the last place of p and of the step taken (fused operations, an
+ * approximate reciprocal).  beta1, beta2, eps and the factors made of them and of
+ * lr are rounded to 32 bits once.  params: B3X_F32 or B3X_BF16; grads:
  * B3X_F32, B3X_BF16 or B3X_F16; each list of one type, each tensor of sizes[k]
  * consecutive elements, tensors apart from one another.  The pointer arrays,
  * sizes and decays are host memory, read before the call returns.
@@ -135,12 +140,15 @@ B3X_TRAIN_API int b3x_train_grad_norm_gpu(int count, const void* const* grads, i
  * moments NaN (with moments in 32 bits its own alone).
  *
  * copies (NULL: none, or NULL entries): bf16 tensors that get the new
- * parameters, rounded to nearest.  decays (NULL: weight_decay for all): a
- * weight decay for each tensor.  grad_scale (NULL: 1) is read on the device;
- * where it is not finite the whole step leaves everything as it was.
+ * parameters, rounded to nearest from 32 bits; parameters that are bf16 and
+ * rounded stochastically differ from their copies by up to one spacing of bf16.
+ * decays (NULL: weight_decay for all): a weight decay for each tensor.
+ * grad_scale (NULL: 1) is read on the device; where it is not finite the whole
+ * step leaves everything as it was.
  * stochastic != 0 rounds what is held in fewer than 32 bits (e4m3 moments, bf16
  * parameters) up or down with probabilities in proportion, by a hash of seed,
- * step, the tensor's place in the list and the element; 0 rounds to nearest. */
+ * step, the tensor's place in the list and the element; 0 rounds to nearest.
+ * Fastest where every array of a tensor starts at a multiple of 4 elements. */
 B3X_TRAIN_API int b3x_train_adamw_gpu(int count, void* const* params, int param_type, const void* const* grads,
         int grad_type, void* const* exp_avg, void* const* exp_avg_sq, float* const* scales, int state_type,
         void* const* copies, const long long* sizes, const float* decays, long long step, double lr,

@@ -144,10 +144,12 @@ __device__ __forceinline__ float warp_most(float x) {
 //
 // 168 M parameters.  In 32 bits throughout 704 us, 6.8 TB/s, a little over the
 // copy rate: bound by memory (bf16 parameters and gradients 558 us, 6.8 TB/s).
-// With 8-bit moments, bf16 parameters and gradients and stochastic rounding 449
-// us, 60% of the copy rate: bound by issued instructions, 81 an element (issue
-// slots 78% busy, the integer pipe 64%), of which the two hashes are 19 and the
-// codes 12.
+// With 8-bit moments, bf16 parameters and gradients and stochastic rounding 451
+// us, 59% of the copy rate: bound by issued instructions, 79 an element (issue
+// slots 77% busy, the integer pipe 63%), of which the two hashes are 19 and the
+// codes 12.  Elements one by one, where any of a tensor's arrays is off a
+// boundary of four: 1,083 us for 731 in 32 bits, 685 for 463 with 8-bit moments
+// (176 M parameters).
 template <class P, class G, bool kF8, bool kRandom, bool kWhole>
 __device__ __forceinline__ void update(const Tensor& t, const Hyper& h, const float gs, const long long base, const int lane) {
     const long long n = t.n;
@@ -490,9 +492,11 @@ int each_list(int count, const long long* sizes, int turns, Fill fill, Go go) {
 }
 
 // Turns of a chunk: one while there are few, so that all SMs have some; then as
-// many as spread a block's start over its work and leave no tail (168 M
-// parameters, with a clip and 32-bit moments: 859 us with one turn, 831 with 4,
-// 845 with 8; with 8-bit moments 541, 460, 449).
+// many as spread a block's start over its work (168 M parameters, with a clip and
+// 32-bit moments: 859 us with one turn, 831 with 4, 845 with 8; with 8-bit
+// moments 541, 460, 449).  Just above the edge 8 turns leave a tail of blocks that
+// fill the SMs in part: 10 M parameters with 8-bit moments 38.2 us, with one turn
+// 34.1; 12 M 42.7 and 39.7; 16 M 51.2 and 52.5; 40 M 114 and 124.
 int turns_for(int count, const long long* sizes, int most) {
     long long all = 0;
     for (int k = 0; k < count; k++) all += sizes[k];

@@ -245,9 +245,9 @@ struct Shared {
 // the one before carried; the blocks of a cluster go through their part once
 // before, for its pair alone (their second reading comes from L2).
 //
-// 64 steps of 4,096 environments side by side: 2.8 us, latency.  256 steps of
+// 64 steps of 4,096 environments side by side: 3.1 us, latency.  256 steps of
 // 16,384: 18 us (4.7 TB/s, 73% of the copy rate).  1,024 environments of up to
-// 8,191 steps one after the other, bf16 values: 34 us (69%), bound by the turns'
+// 8,191 steps one after the other, bf16 values: 34 us (68%), bound by the turns'
 // chains of loads and joins at 64 registers a thread; loading a turn ahead took
 // registers and 46 us (at 4 steps a thread, where this took 39).  65,536 steps
 // of one environment: 13 us on a cluster's eight SMs.

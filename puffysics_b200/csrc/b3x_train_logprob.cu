@@ -294,14 +294,22 @@ __device__ __noinline__ float2 far_sums(const Source<T, kMask>& src, float m, fl
 //
 // Alternatives: a threshold that K logits reach, then what reaches it is ranked.
 // With 32 lanes it is the K-th largest of the lanes' maxima, with fewer that of
-// the vectors'.
+// the vectors'; where there are fewer vectors than alternatives it is no
+// threshold at all.  A row has room for 8 candidates a lane.  More than that
+// takes K passes over the row, and it is the rule, not the exception, with more
+// alternatives than vectors (16-bit rows of 17 to 128 logits with 20, of 17 to
+// 256 with 32) as with 29 and more of 32 maxima, which some 70 to 130 logits
+// reach: 65,536 bf16 rows of 50 logits with 20 alternatives 106 us, of 100 183
+// us, of 200 61 us and with 32 alternatives 468 us, of 1,000 with 32 384 us.
 //
 // Lanes by the row's length, so that a lane has up to 4 vectors in flight and the
 // reductions and a row's last steps (a logarithm, a division, its stores) are
 // shared by as few as will do.  Bound by issued instructions and by latency, not
 // by memory: 147,456 masked rows of 21 f32 with the greedy action 8.5 us (the
 // bytes alone 3.1), 65,536 rows of 1,000 bf16 45 us (20.6), with 20 alternatives
-// 103.  Without alternatives five blocks an SM (four 49 us); with them four.
+// 104.  Without alternatives five blocks an SM (four 49 us); with them four.
+// At 48 and 64 registers a thread the 16-bit forms spill: up to 40 bytes without
+// alternatives, 96 to 144 with them.
 constexpr int kRowThreads = 256;
 constexpr int kRowFound = 256;       // logits that are ranked at once, for a warp's rows together
 
@@ -464,7 +472,8 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 4 : 5) lanes_kernel(Rows a
             entries[here][i] = entry_of(key_of(to_float(src.row[j])), j);
         }
     } else if (L == 32 && p.m == p.m) {
-        // many logits, by far the most equal to the threshold: all above it, then the first of those
+        // more than are ranked at once, as where many are equal to the threshold and with 31 or 32 alternatives: all above
+        // it, then the first of those that are equal to it
         const uint32_t key = key_of(z);
         __syncwarp();
         if (lane == 0) found[here] = 0;
@@ -496,7 +505,7 @@ __global__ void __launch_bounds__(kRowThreads, kTop ? 4 : 5) lanes_kernel(Rows a
         for (int i = n + lane; i < o.top; i += L) write_top(o, row, i, 0, r, a.scale);
     }
     if (__all_sync(~0u, ranked)) return;
-    // too many logits to rank, or NaN: each time the best one after the last
+    // more logits than there is room for, or NaN: each time the best one after the last
     uint64_t last = ~0ull;
     for (int k = 0; k < o.top; k++) {
         uint64_t top = 0;
@@ -667,12 +676,13 @@ __device__ __noinline__ void crowded(const Source<T, kMask>& src, Shared& sh, in
 // from L2.
 //
 // 4,096 rows of 131,072 bf16: 177 us without alternatives (6.1 TB/s, 94% of the
-// copy rate), 217 with 20 (77%).  An exponential a logit keeps the special
+// copy rate), 215 to 219 with 20 (77%).  An exponential a logit keeps the special
 // function unit half busy; the rest of the time is the loads' latency at 64
 // registers a thread, and each row's end (sorting, ranking), which other blocks
 // of the SM cover in part.  12 blocks an SM instead of 8 spill (267 us).  8 rows,
-// a cluster of 8 blocks each: 4.7 us without alternatives, 9.6 with 20, all of it
-// latency.
+// a cluster of 8 blocks each: 4.7 us without alternatives, 9.7 with 20, all of it
+// latency; kOnce with alternatives spills 100 bytes a thread at 64 registers.  Rows
+// that are out of range are read a second time (4,096 rows all of -1e9: 488 us).
 template <class T, bool kMask, bool kTop, bool kOnce, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallBlocks) long_kernel(Rows a, Out o, int cluster, int shift) {
     __shared__ Shared sh;
@@ -835,7 +845,7 @@ static_assert(kMaxCluster * B3X_TRAIN_MAX_TOP <= kFound, "the blocks' alternativ
 template <class T, bool kMask, bool kTop>
 int launch_long(const Rows& a, const Out& o, int nv, cudaStream_t s) {
     // A cluster a row while rows alone leave SMs idle and each block keeps 1,024 vectors: 8 rows of 131,072 bf16 with 20
-    // alternatives 9.6 us, by single blocks 13.5; 8 rows of 32,768 8.1 us so, by two blocks each 10.2.
+    // alternatives 9.7 us, by single blocks 13.5; 8 rows of 32,768 8.1 us so, by two blocks each 10.2.
     int cluster = 1;
     while (cluster < kMaxCluster && a.rows * cluster * 2 <= 296 && nv / (cluster * 2) >= 1024) cluster *= 2;
     int each = (nv + cluster - 1) / cluster;

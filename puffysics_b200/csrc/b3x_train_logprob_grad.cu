@@ -27,8 +27,11 @@ constexpr int kMaxCluster = 8;
 
 // 2^bits threads a row (a cluster's blocks together where it has more than one),
 // 16 bytes of logits and of gradients at a time; bound by memory (2,048 rows of
-// 65,536 bf16: 92 us, 5.8 TB/s, 91% of the copy rate; 4,096 rows of 50,001: 156
-// us, 81%; masked 61%, by the mask's instructions).  With
+// 65,536 bf16: 92 us, 5.8 TB/s, 90% of the copy rate; 4,096 rows of 50,001: 157
+// us, 81%; 2,048 masked rows of 50,001 f16 131 us, 60%: every vector's mask is
+// two or three loads of a word and their shifts).  Gradients at another place
+// modulo 16 bytes than their logits are stored one by one (500 us for the 157 of
+// 4,096 rows of 50,001).  With
 // e = log p_j the gradient is p_j (B e + A) with A = -scale (g + h H) and
 // B = -scale h, and scale g more at the action.
 template <class T, bool kMask>

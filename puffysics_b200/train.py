@@ -11,6 +11,12 @@ given to a call is in use on its stream until the work is done, as with any
 kernel: a tensor that another stream made or will free has to be ordered by the
 caller.  There is no CPU path: loading fails loudly when a library is missing.
 
+The calls read and write memory and are not part of autograd: outputs carry no
+graph and their version counters stay, so a loss made of logprob's outputs gives
+the logits no gradient.  Take the derivatives by logp and entropy to
+logprob_grad, and its result to backward() (examples/hover_train.py); and do not
+let a call overwrite what autograd has saved, which it would not notice.
+
 The checks are made in compiled code (csrc/b3x_train_py.cpp): made in Python
 they took as long as a launch.
 
@@ -142,7 +148,8 @@ def adamw(params, grads, exp_avg, exp_avg_sq, step, lr, beta1=0.9, beta2=0.999, 
     weight_decay: a number, or a list with one for each tensor.  grad_scale: a
     float32 tensor of one element (grad_norm's out[1:]); where it is not finite
     the step changes nothing.  copies: bfloat16 tensors that get the new
-    parameters.  seed: round 8-bit moments and bfloat16 parameters
+    parameters rounded to nearest (also where bfloat16 parameters themselves are
+    rounded stochastically).  seed: round 8-bit moments and bfloat16 parameters
     stochastically by this 32-bit number; None rounds to nearest."""
     return _binding().adamw(params, grads, exp_avg, exp_avg_sq, step, lr, beta1, beta2, eps, weight_decay, scales,
                             grad_scale, copies, seed, *_place(stream))
