@@ -46,8 +46,8 @@ __device__ __forceinline__ float factor_of(const Rows& a) { return fminf(a.scale
 // Joined parts move to the larger r: 2^(x + d) (x + d) = 2^d (2^x x + d 2^x).
 // Shifts and exponents stop at -1e4, where 2^x is 0 already, so that -infinity
 // never meets a zero factor.  From |c m| = 2^24 on, whole numbers that floats
-// hold are not always near c m: a row with such a maximum is summed about the
-// maximum itself, and a part with one (a stretch filled with -1e9, say), whose
+// hold are not always near c m: a row whose maximum has none is summed about the
+// maximum itself, and a part of such logits (a stretch filled with -1e9, say), whose
 // sums may be beyond the floats, is dropped where 2^d is 0: in any other row it
 // weighs nothing.  A NaN maximum stays; sums beside it mean nothing.
 struct Part {
@@ -76,10 +76,13 @@ __device__ __forceinline__ Part join_lanes(Part a) {
     return a;
 }
 
-// Whether no whole number is near c m (|c m| of 2^24 and more, or beyond the
-// floats): the row needs sums of (z - m) instead.
+// Whether no whole number is near enough to c m (possible from 2^24 on): the row
+// needs sums of (z - m) instead.  Up to 40 above r the sums lose nothing but what
+// ln s and ln 2 t / s, of up to 28 each, cost the entropy in their last places;
+// below r by more than 2 a dropped part could weigh something.
 __device__ __forceinline__ bool out_of_range(const Part& a, float c) {
-    return fabsf(a.m) < kInf && !(fabsf(__fmaf_rn(a.m, c, -a.r)) <= 1.0f);
+    const float x = __fmaf_rn(a.m, c, -a.r);
+    return fabsf(a.m) < kInf && !(x >= -2.0f && x <= 40.0f);
 }
 
 constexpr float kLn2 = 0.6931471805599453f;
@@ -682,7 +685,7 @@ __device__ __noinline__ void crowded(const Source<T, kMask>& src, Shared& sh, in
 // of the SM cover in part.  12 blocks an SM instead of 8 spill (267 us).  8 rows,
 // a cluster of 8 blocks each: 4.7 us without alternatives, 9.7 with 20, all of it
 // latency; kOnce with alternatives spills 100 bytes a thread at 64 registers.  Rows
-// that are out of range are read a second time (4,096 rows all of -1e9: 488 us).
+// that are out of range are read a second time (4,096 rows all of -1e10: 488 us).
 template <class T, bool kMask, bool kTop, bool kOnce, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, kWarps == kMaxWarps ? 2 : kSmallBlocks) long_kernel(Rows a, Out o, int cluster, int shift) {
     __shared__ Shared sh;
